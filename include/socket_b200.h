@@ -451,6 +451,66 @@ SK_API int sk_pick_token(const void* logits, int dtype, int64_t ld, int batch, i
 SK_API int sk_begin_token(const int64_t* first, int64_t* token, int batch, int64_t* pos, int32_t* seqlens, int64_t position,
                           int32_t* const* lengths, int n, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * A key-value cache in pages: pools [n_pages, G, page, D] of keys and of values (rows of D elements; strides in elements,
+ * rows k_rs apart, heads k_hs, pages k_ps, and v_rs, v_hs, v_ps), a table [B, width] of page numbers (rows table_ld apart)
+ * and lengths [B].  Slot j of sequence b is row j % page of page table[b, j / page]; a sequence has at most width * page
+ * slots, of which the first lengths[b] are in use (a negative length counts as 0).  Optional, per sequence, key/value head
+ * and slot: mass (fp32, the attention weight a key has collected) and positions (int32, its token's position), heads
+ * mass_hs / pos_hs and sequences mass_bs / pos_bs elements apart.
+ * page is a power of two, at least 16; D a multiple of 8 (bf16, fp16) or 4 (fp32), at most 256.  Pools and their strides
+ * are 16-byte aligned.  Sequences may share pages that are only read; a page that a call writes belongs to one sequence.
+ * A slot behind the last is not touched (SK_DEV_POS_OUT_OF_RANGE), nor is a page outside [0, n_pages)
+ * (SK_DEV_INDEX_OUT_OF_RANGE): its keys are left out. */
+typedef struct sk_paged_cache {
+    void* k;
+    void* v;
+    const int32_t* table;
+    const int32_t* lengths;
+    float* mass;
+    int32_t* positions;
+    int32_t* status;
+    int64_t k_ps, k_hs, k_rs, v_ps, v_hs, v_rs, table_ld, n_pages, mass_bs, mass_hs, pos_bs, pos_hs;
+    int dtype, B, G, D, page, width;
+} sk_paged_cache;
+
+/* New keys and values [B, S, G, D] (strides: sequence, token, head) into slots lengths[b] .. lengths[b] + counts[b] - 1 of
+ * every sequence; counts NULL: S each (counts are cut to [0, S]).  mass, if any, starts at 0 there; positions, if any, are
+ * first[b] + token (first NULL: the slot itself).  lengths is not advanced. */
+SK_API int sk_paged_append(const sk_paged_cache* c, const void* k_new, int64_t kn_bs, int64_t kn_ss, int64_t kn_hs,
+                           const void* v_new, int64_t vn_bs, int64_t vn_ss, int64_t vn_hs, int S, const int32_t* counts,
+                           const int32_t* first, void* stream);
+
+/* Softmax attention of one query token per sequence, q [B, H, D] (heads q_hs, sequences q_bs apart; H a multiple of G,
+ * query heads of one key/value head in a row), over the first lengths[b] + extra slots: out [B, H, D] in q's type (that of
+ * the pools), scores scale * q.k, all sums in fp32.  No key: zeros.  With mass, every attended slot of (b, g) is increased by
+ * the sum of its weights over the query heads of g.  No atomics: the result does not depend on the order blocks run in.
+ * `workspace`: sk_paged_attn_workspace_bytes of the same cache and H, overwritten by every call. */
+SK_API size_t sk_paged_attn_workspace_bytes(const sk_paged_cache* c, int H);
+SK_API int sk_paged_attn(const sk_paged_cache* c, const void* q, int64_t q_bs, int64_t q_hs, void* out, int64_t o_bs, int64_t o_hs,
+                         int H, int extra, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Cuts every sequence longer than `budget` to `budget` slots, for each key/value head by itself: kept are the slots whose
+ * position is below `sink`, those within the last `recent` positions up to the head's largest, and of the others those with
+ * the largest mass (NaN above all, the lowest slot of equal ones).  Kept slots below `budget` stay where they are; the i-th
+ * kept slot from `budget` on moves into the i-th freed one.  Requires sink + recent <= budget, budget >= 1, mass and
+ * positions.  mass_out / pos_out [B, G, width * page] (strides as theirs; may be mass and positions) get the new values, 0
+ * and -1 behind the new length; lengths_out[b] (may be lengths) = the smaller of the budget and the slots in use.  Keys and values move in place.
+ * A slot whose page is outside the pool takes part, but no row of it is moved. */
+SK_API size_t sk_paged_evict_workspace_bytes(const sk_paged_cache* c, int budget);
+SK_API int sk_paged_evict(const sk_paged_cache* c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs,
+                          int32_t* pos_out, int64_t po_bs, int64_t po_hs, int32_t* lengths_out, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* How likely tokens were: of logits [rows, vocab] (rows ld elements apart) logprob[r] = log softmax(logits[r])[token[r]]
+ * (token may be NULL, then logprob is not written), entropy[r] (or NULL) of the whole row in nats, and the `top` largest logits
+ * with their log probabilities, largest first, the lower index first of equal ones (NaN before all, as sk_pick_token):
+ * top_logprob, top_token [rows, top].  0 <= top <= min(64, vocab).  fp32 sums.  Logits of -inf have probability 0 and add
+ * nothing to the entropy; a row with NaN or +inf, or of -inf alone, has NaN log probabilities and entropy.  A token outside
+ * [0, vocab) has log probability NaN and sets SK_DEV_INDEX_OUT_OF_RANGE. */
+SK_API int sk_token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int vocab, const int64_t* token, int top,
+                             float* logprob, float* entropy, float* top_logprob, int64_t* top_token, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

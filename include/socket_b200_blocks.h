@@ -60,6 +60,10 @@ SK_API int skb_residual_norm(const sk_residual_params* p, void* stream);
 SK_API int skb_linear_rows_applicable(const sk_linear_params* p);
 SK_API int skb_linear_rows(const sk_linear_params* p, void* stream);
 
+/* How likely tokens were, as sk_token_logprobs of socket_b200.h. */
+SK_API int skb_token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int vocab, const int64_t* token, int top,
+                              float* logprob, float* entropy, float* top_logprob, int64_t* top_token, int32_t* status, void* stream);
+
 /* The end of a greedy decode step, as sk_pick_token of socket_b200.h. */
 SK_API int skb_pick_token(const void* logits, int dtype, int64_t ld, int batch, int vocab, int64_t* token, int64_t* pos,
                           int32_t* seqlens, void* stream);

@@ -55,6 +55,16 @@ class LinearParams(C.Structure):
     ]
 
 
+class PagedCacheParams(C.Structure):
+    """Mirror of `sk_paged_cache`."""
+    _fields_ = [
+        ("k", _p), ("v", _p), ("table", _p), ("lengths", _p), ("mass", _p), ("positions", _p), ("status", _p),
+        ("k_ps", _i64), ("k_hs", _i64), ("k_rs", _i64), ("v_ps", _i64), ("v_hs", _i64), ("v_rs", _i64), ("table_ld", _i64),
+        ("n_pages", _i64), ("mass_bs", _i64), ("mass_hs", _i64), ("pos_bs", _i64), ("pos_hs", _i64),
+        ("dtype", _i), ("B", _i), ("G", _i), ("D", _i), ("page", _i), ("width", _i),
+    ]
+
+
 # name -> (restype, argtypes); the order follows include/socket_b200.h
 SIGNATURES = {
     "sk_abi_version": (_i, []),
@@ -106,6 +116,12 @@ SIGNATURES = {
     "sk_rms_norm": (_i, [_p, _p, _i, _i64, _i, _f, _p, _p]),
     "sk_pick_token": (_i, [_p, _i, _i64, _i, _i, _p, _p, _p, _p]),
     "sk_begin_token": (_i, [_p, _p, _i, _p, _p, _i64, _p, _i, _p]),
+    "sk_paged_append": (_i, [C.POINTER(PagedCacheParams), _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _p, _p, _p]),
+    "sk_paged_attn_workspace_bytes": (_sz, [C.POINTER(PagedCacheParams), _i]),
+    "sk_paged_attn": (_i, [C.POINTER(PagedCacheParams), _p, _i64, _i64, _p, _i64, _i64, _i, _i, _f, _p, _sz, _p]),
+    "sk_paged_evict_workspace_bytes": (_sz, [C.POINTER(PagedCacheParams), _i]),
+    "sk_paged_evict": (_i, [C.POINTER(PagedCacheParams), _i, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _sz, _p]),
+    "sk_token_logprobs": (_i, [_p, _i, _i64, _i64, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
 }
 
 
@@ -181,6 +197,7 @@ BLOCK_SIGNATURES = {
     "skb_residual_norm": (_i, [C.POINTER(ResidualParams), _p]),
     "skb_linear_rows_applicable": (_i, [C.POINTER(LinearParams)]),
     "skb_linear_rows": (_i, [C.POINTER(LinearParams), _p]),
+    "skb_token_logprobs": (_i, [_p, _i, _i64, _i64, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
     "skb_pick_token": (_i, [_p, _i, _i64, _i, _i, _p, _p, _p, _p]),
     "skb_begin_token": (_i, [_p, _p, _i, _p, _p, _i64, _p, _i, _p]),
     "skb_glu": (_i, [_p, _p, _i, _i64, _i, _i64, _i, _f, _f, _p, _i64, _p]),
@@ -257,6 +274,15 @@ def stream_ptr(device=None) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = None if device is None else device.index
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def on_device(device: torch.device, check_status, entry, what: str, *args) -> None:
+    """entry(*args, stream) on the current stream of `device`, whichever device is the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        check_status(entry(*args, stream_ptr(device)), what)
+        return
+    with torch.cuda.device(device):
+        check_status(entry(*args, stream_ptr(device)), what)
 
 
 def dtype_code(t: torch.Tensor) -> int:

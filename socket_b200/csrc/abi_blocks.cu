@@ -119,6 +119,11 @@ int skb_pick_token(const void* logits, int dtype, int64_t ld, int batch, int voc
     return pick_token(logits, dtype, ld, batch, vocab, token, pos, seqlens, (cudaStream_t)stream);
 }
 
+int skb_token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int vocab, const int64_t* token, int top,
+                       float* logprob, float* entropy, float* top_logprob, int64_t* top_token, int32_t* status, void* stream) {
+    return token_logprobs(logits, dtype, ld, rows, vocab, token, top, logprob, entropy, top_logprob, top_token, status, (cudaStream_t)stream);
+}
+
 int skb_begin_token(const int64_t* first, int64_t* token, int batch, int64_t* pos, int32_t* seqlens, int64_t position,
                     int32_t* const* lengths, int n, void* stream) {
     return begin_token(first, token, batch, pos, seqlens, position, lengths, n, (cudaStream_t)stream);

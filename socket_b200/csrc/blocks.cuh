@@ -119,6 +119,8 @@ int pick_token(const void* logits, int dtype, int64_t ld, int batch, int vocab, 
                cudaStream_t st);                                         // the same
 int begin_token(const int64_t* first, int64_t* token, int batch, int64_t* pos, int32_t* seqlens, int64_t position, int32_t* const* lengths,
                 int n, cudaStream_t st);                                 // the same
+int token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int vocab, const int64_t* token, int top, float* logprob,
+                   float* entropy, float* top_logprob, int64_t* top_token, int32_t* status, cudaStream_t st);      // the same
 int rms_norm_rows(const void* x, const void* w, int dtype, int64_t rows, int width, float eps, void* out, cudaStream_t st);
 int launch_glu(const void* gate, const void* up, int dtype, int64_t rows, int ff, int64_t ld, int kind, float limit, float slope,
                void* out, int64_t out_ld, cudaStream_t st);

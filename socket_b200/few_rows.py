@@ -1,20 +1,21 @@
 """Operators on the few rows of a decode step that every decoder uses: projections that stream the weights once, an RMS
-norm of rows in the model's type, the greedy pick.  Both libraries hold the projections and the pick, the step library
-the norm; a model calls those of the library it is built on (`library`: "step" or "blocks")."""
+norm of rows in the model's type, the greedy pick, log probabilities of tokens.  Both libraries hold the projections, the pick and the log
+probabilities, the step library the norm; a model calls those of the library it is built on (`library`: "step" or "blocks")."""
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import blocks, check, check_blocks, dtype_code, lib, ptr, stream_ptr
+from ._lib import blocks, check, check_blocks, dtype_code, lib, on_device, ptr, stream_ptr
 from .ops import _require_cuda
 
 GLU_CLAMPED, GLU_SILU = 0, 1
 FEW_ROWS = 8                # the most that the streaming projection takes
+TOP_TOKENS = 64             # the most alternatives of `token_logprobs`
 
 
 def _call(library: str, name: str, *args) -> int:
@@ -115,6 +116,40 @@ def pick_token(logits: Tensor, token: Tensor, pos: Tensor, seqlens: Tensor, libr
     logits = _separate_rows(logits)                               # lives until the launch
     _launch(library, "pick_token", ptr(logits), dtype_code(logits), _ld(logits), logits.shape[0], logits.shape[1], ptr(token), ptr(pos),
             ptr(seqlens), stream_ptr(logits.device))
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: Optional[Tensor]          # [rows] log probability of the given tokens
+    entropy: Tensor                     # [rows] of the whole distribution, in nats
+    top_logprobs: Tensor                # [rows, top] of the likeliest tokens, likeliest first
+    top_tokens: Tensor                  # [rows, top]
+
+
+def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int = 0, status: Optional[Tensor] = None,
+                   library: str = "step") -> TokenLogprobs:
+    """How likely `tokens` (int64, one per row, or None) were under logits [rows, vocab] (any number of rows), with the entropy
+    of every row and its `top` (at most 64) likeliest tokens, the lower index first of equal ones.  fp32; logits are read once.  A
+    row of nothing but -inf, or with NaN or +inf, gives NaN; so does a token outside the vocabulary, which also flags `status`."""
+    _require_cuda(logits)
+    dev = logits.device
+    _require_on(dev, tokens, status)
+    assert logits.dim() == 2
+    rows, vocab = logits.shape
+    if not 0 <= top <= min(TOP_TOKENS, vocab):
+        raise RuntimeError(f"token_logprobs: {top} alternatives of {vocab} tokens (at most {TOP_TOKENS})")
+    logits = _separate_rows(logits)                               # lives until the launch
+    found = torch.empty(2 + top, rows, dtype=torch.float32, device=dev)
+    logprobs, entropy, top_logprobs = found[0], found[1], found[2:].view(rows, top)
+    top_tokens = torch.empty(rows, top, dtype=torch.int64, device=dev)
+    if tokens is None:
+        logprobs = None
+    else:
+        assert tokens.dtype == torch.int64 and tokens.numel() == rows
+        tokens = tokens.contiguous()
+    entry = lib().sk_token_logprobs if library == "step" else blocks().skb_token_logprobs
+    on_device(dev, check if library == "step" else check_blocks, entry, "token_logprobs", logits.data_ptr(), dtype_code(logits), _ld(logits), rows,
+              vocab, ptr(tokens), top, ptr(logprobs), entropy.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr(), ptr(status))
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)
 
 
 def begin_token(first: Tensor, token: Tensor, pos: Tensor, seqlens: Tensor, position: int, lengths: Sequence[Tensor], library: str) -> None:
