@@ -1,53 +1,525 @@
-// Softmax attention of one new token per sequence over a paged cache.
+// Softmax attention of one new token per sequence over a paged cache, split over the keys and joined.
+//
+//   out_h = sum_j w_hj v_j,  w_hj = exp(s_hj - m_h) / l_h,  s_hj = scale q_h . k_j,  m_h = max_j s_hj,  l_h = sum_j exp(s_hj - m_h)
+//
+// in one pass over the keys with a running maximum, and mass_j += sum over the head's queries of w_hj.  Bound by the bytes of
+// keys and values: 2 D elements a key, each read once for all query heads of its key/value head.
+//
+// Work: all keys of all (sequence, key/value head) pairs stand in one row of chunks of WARPS x 16 keys, and every block takes an
+// equal run of it, so that ragged batches load the SMs evenly.  A warp works by itself on its 16 keys of a chunk - 16 keys never
+// leave a page - with three stages of asynchronous copies of its own and no block barrier.  Only where a run crosses into the next
+// pair, or ends, the block's warps join; a pair inside one run is then finished, others leave a partial result for a second kernel.
+// The second kernel also adds the weights to mass, from scores that the first one leaves behind (they need the final maximum and sum).
+//
+// 16-bit types: S^T = K Q^T and O^T = V^T P^T by m16n8k16 products, keys and then value columns in the 16 rows and up to 8 query heads in
+// the 8 columns, which wastes half of what heads in the rows would.  Weights go in as two halves (value and rounding rest), so that what is
+// added up has 16 bits of each weight.  fp32: fused multiply-adds, a lane per key for scores, a lane per four columns for values.
 #include "paged.cuh"
+#include "warp_mma.cuh"
 
 namespace sk {
 namespace {
 
-// One block per (sequence, key/value head), its query heads one after the other: a warp takes every eighth key, its lanes the head's
-// elements; running maximum and sums per warp, joined at the end.  With mass the scores are taken a second time once maximum and
-// sum are known.
-constexpr int PT_WARPS = 8;
-template <typename T>
-__global__ void __launch_bounds__(PT_WARPS * 32)
-paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const T* q, int64_t q_bs, int64_t q_hs, T* out, int64_t o_bs, int64_t o_hs, int H,
-                  int extra, float scale) {
-    constexpr int E = 8;                                       // elements of a head per lane: 256 / 32
-    __shared__ float ms[PT_WARPS], ls[PT_WARPS], os[PT_WARPS][256];
-    const int g = blockIdx.x % c.G, b = blockIdx.x / c.G, rep = H / c.G;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shift = 31 - __clz(c.page);
-    bool over;
-    const int n = paged_length(c, b, extra, &over);
-    if (over && threadIdx.x == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
-    for (int h = g * rep; h < (g + 1) * rep; ++h) {
-        float x[E], o[E], m = -INFINITY, l = 0.f;
+constexpr float PT_LOG2E = 1.4426950408889634f;
+constexpr int PT_KEYS = 16;                                    // keys of a warp's tile
+
+template <typename T, int DP_, int NT_> struct PtShape {
+    static constexpr int DP = DP_, NT = NT_;                   // head size padded, groups of heads
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int HG = (F32 ? 4 : 8) * NT;              // query heads of a block
+    static constexpr int ROW = DP * (int)sizeof(T), HALF = PT_KEYS * ROW, TILE = 2 * HALF;
+    static constexpr int WARPS = TILE <= 8192 ? 8 : 65536 / TILE, STAGES = !F32 && NT == 2 ? 2 : 3;
+    static constexpr int CHUNK = WARPS * PT_KEYS, THREADS = WARPS * 32;
+    static constexpr int OS = DP + 4;                          // row of the joined sums: columns of four query pairs in four bank groups
+    static constexpr size_t SMEM = (size_t)WARPS * STAGES * TILE + (size_t)WARPS * HG * OS * 4 + (F32 ? (size_t)HG * DP * 4 + (size_t)WARPS * PT_KEYS * HG * 4 : 0);
+    static constexpr int PER_SM = SMEM <= 112 * 1024 ? 2 : 1;
+    static_assert(SMEM <= 226 * 1024, "shared memory of a block");
+};
+
+struct PtArgs {
+    const void* q;
+    void* out;
+    float *parts, *stats, *scores;                             // partial results; final maximum and 1 / sum per head; scores for mass
+    int64_t q_bs, q_hs, o_bs, o_hs;
+    int H, extra, groups, rs;                                  // groups of HG heads per key/value head; scores of a key
+    float scale;                                               // times log2(e)
+};
+
+// Sum over the block, `red` of one value per warp; every thread gets it
+__device__ __forceinline__ int64_t pt_block_sum(int64_t v, int64_t* red) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = lane + 32 * e;
-            x[e] = d < c.D ? to_f32(q[b * q_bs + h * q_hs + d]) : 0.f;
-            o[e] = 0.f;
+    for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v += red[w];
+    __syncthreads();
+    return v;
+}
+
+__device__ __forceinline__ uint32_t pt_turn(uint32_t x) {      // an 8 x 8 matrix of 16-bit elements, transposed
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pt_pack(float x, float y);
+template <> __device__ __forceinline__ uint32_t pt_pack<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pt_pack<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ float pt_low(uint32_t x);
+template <> __device__ __forceinline__ float pt_low<__nv_bfloat16>(uint32_t x) { return __uint_as_float(x << 16); }
+template <> __device__ __forceinline__ float pt_low<__half>(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)x)); }
+template <typename T> __device__ __forceinline__ float pt_high(uint32_t x);
+template <> __device__ __forceinline__ float pt_high<__nv_bfloat16>(uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); }
+template <> __device__ __forceinline__ float pt_high<__half>(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)(x >> 16))); }
+
+// exp2(a - b) with exp2(-inf - -inf) = 0
+__device__ __forceinline__ float pt_factor(float a, float b) { return exp2_fast(a - (b == -INFINITY ? 0.f : b)); }
+__device__ __forceinline__ float pt_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// A place in the row of chunks: chunk `chunk` of `chunks` of pair `unit` of sequence b, which has n keys
+struct PtPlace {
+    int b, unit, chunk, chunks, n;
+};
+
+template <typename S, typename T>
+__global__ void __launch_bounds__(S::THREADS, S::PER_SM)
+paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constant__ PtArgs a) {
+    pdl_begin();
+    constexpr int DP = S::DP, HG = S::HG, WARPS = S::WARPS, STAGES = S::STAGES, CHUNK = S::CHUNK, VE = 16 / (int)sizeof(T), OS = S::OS;
+    constexpr int PIECES = S::ROW / 16;                        // 16-byte pieces of a row
+    extern __shared__ __align__(1024) char pt_smem[];
+    __shared__ int64_t red[WARPS];
+    __shared__ float ms[WARPS][HG], ls[WARPS][HG];
+    __shared__ PtPlace start_s;
+    char* tiles = pt_smem + (threadIdx.x >> 5) * STAGES * S::TILE;                                  // [stage][keys | values][16][ROW]
+    float* os = reinterpret_cast<float*>(pt_smem + WARPS * STAGES * S::TILE);                       // [WARPS][HG][OS]
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, shift = 31 - __clz(c.page);
+    const int units = c.G * a.groups, rep = a.H / c.G;
+    auto chunks_of = [](int n) { return (n + CHUNK - 1) / CHUNK; };
+
+    // ---- this block's run of chunks
+    int64_t total = 0;
+    for (int b = t; b < c.B; b += S::THREADS) {
+        bool over;
+        total += chunks_of(paged_length(c, b, a.extra, &over));
+        if (over && blockIdx.x == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
+    }
+    total = pt_block_sum(total, red) * units;
+    for (int b = blockIdx.x; b < c.B; b += gridDim.x)          // no key, no run: zeros
+        if (paged_length(c, b, a.extra) == 0)
+            for (int i = t; i < a.H * c.D; i += S::THREADS) ((T*)a.out)[b * a.o_bs + i / c.D * a.o_hs + i % c.D] = from_f32<T>(0.f);
+    const int64_t per = (total + gridDim.x - 1) / gridDim.x, first = per * blockIdx.x;
+    int left = (int)max(min(per, total - first), (int64_t)0);
+    if (left == 0) return;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < c.B; b0 += S::THREADS) {             // the sequence that holds chunk `first`
+        const int b = b0 + t, n = b < c.B ? paged_length(c, b, a.extra) : 0, m = chunks_of(n);
+        int64_t sum = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(FULL, sum, o);
+            if (lane >= o) sum += x;
         }
-        auto score = [&](int j, int page) {
-            const T* k = (const T*)c.k + page * c.k_ps + g * c.k_hs + (j & (c.page - 1)) * c.k_rs;
-            float s = 0.f;
+        if (lane == 31) red[warp] = sum;
+        __syncthreads();
+        int64_t all = 0;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) sum += red[w];
+            all += red[w];
+        }
+        const int64_t lo = (before + sum - m) * units, hi = (before + sum) * units;
+        if (lo <= first && first < hi) start_s = PtPlace{b, (int)((first - lo) / m), (int)((first - lo) % m), m, n};
+        before += all;
+        __syncthreads();
+        if (before * units > first) break;
+    }
+    PtPlace cur = start_s, ld = cur;
+    auto step = [&](PtPlace& p) {
+        if (++p.chunk < p.chunks) return;
+        p.chunk = 0;
+        if (++p.unit < units) return;
+        p.unit = 0;
+        do {
+            p.n = ++p.b < c.B ? paged_length(c, p.b, a.extra) : 1;
+        } while (p.n == 0);
+        p.chunks = chunks_of(p.n);
+    };
+
+    // ---- copies: this warp's tile of the chunk at `ld`, one commit group each; `live` has a bit per stage that holds keys
+    int ld_left = left, ld_stage = 0, ld_page = 0;
+    uint32_t live = 0;
+    auto ask_page = [&]() {
+        const int j = ld.chunk * CHUNK + warp * PT_KEYS;
+        if (ld_left > 0 && j < ld.n) ld_page = __ldcg(c.table + ld.b * c.table_ld + (j >> shift));
+    };
+    auto issue = [&]() {
+        live &= ~(1u << ld_stage);
+        if (ld_left > 0) {
+            const int j = ld.chunk * CHUNK + warp * PT_KEYS, rows = ld.n - j;
+            if (rows > 0) {
+                if (paged_page_ok(c, ld_page)) {
+                    const int g = ld.unit / a.groups;
+                    const T* k = (const T*)c.k + ld_page * c.k_ps + g * c.k_hs + (j & (c.page - 1)) * c.k_rs;
+                    const T* v = (const T*)c.v + ld_page * c.v_ps + g * c.v_hs + (j & (c.page - 1)) * c.v_rs;
+                    const uint32_t dst = saddr(tiles + ld_stage * S::TILE);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (lane + 32 * e < c.D) s = fmaf(x[e], to_f32(k[lane + 32 * e]), s);
-            return warp_sum(s) * scale;
-        };
-        for (int j = warp; j < n; j += PT_WARPS) {
-            const int page = c.table[b * c.table_ld + (j >> shift)];
-            if (!paged_page_ok(c, page)) {
-                if (lane == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
-                continue;
+                    for (int i = 0; i < PT_KEYS * PIECES / 32; ++i) {
+                        const int x = i * 32 + lane, r = x / PIECES, p = x % PIECES;
+                        const bool in = r < rows && p * VE < c.D;      // others are zeros
+                        const uint32_t at = dst + r * S::ROW + ((p ^ (r & 7)) << 4);
+                        cp16(at, in ? k + r * c.k_rs + p * VE : k, in);
+                        cp16(at + S::HALF, in ? v + r * c.v_rs + p * VE : v, in);
+                    }
+                    live |= 1u << ld_stage;
+                } else if (lane == 0 && c.status != nullptr) {
+                    atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
+                }
             }
-            const float s = score(j, page), mn = fmaxf(m, s);
-            const float mc = mn == -INFINITY ? 0.f : mn, f = expf(m - mc), w = expf(s - mc);      // a NaN score is a NaN weight
-            const T* v = (const T*)c.v + page * c.v_ps + g * c.v_hs + (j & (c.page - 1)) * c.v_rs;
+            --ld_left;
+            if (ld_left > 0) step(ld);
+            ask_page();
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ld_stage = ld_stage + 1 == STAGES ? 0 : ld_stage + 1;
+    };
+    ask_page();
+    for (int s = 0; s < STAGES - 1; ++s) issue();
+
+    // ---- queries of a pair, running maxima and sums
+    constexpr int KK = DP / 16, NT = S::NT;
+    constexpr int CPL = S::F32 ? (DP / 4 + 31) / 32 : 1;       // fp32: 16-byte pieces of a value row per lane
+    uint32_t qf[S::F32 ? 1 : NT][S::F32 ? 1 : KK][2];
+    float acc[S::F32 ? HG : KK][S::F32 ? CPL : NT][4];         // 16 bit: rows of value columns x heads; fp32: heads x columns
+    constexpr int MC = S::F32 ? HG : 2 * NT;                   // heads whose maximum a lane keeps
+    float m[MC], l[MC];
+    float* qs = os + WARPS * HG * OS;                          // fp32: [HG][DP] queries, [WARPS][16][HG] weights
+    float* ps = qs + HG * DP + warp * PT_KEYS * HG;
+    auto begin = [&]() {
+        const int g = cur.unit / a.groups, h0 = g * rep + cur.unit % a.groups * HG, heads = min(HG, (g + 1) * rep - h0);
+        const T* q = (const T*)a.q + cur.b * a.q_bs + h0 * a.q_hs;
+        if constexpr (S::F32) {
+            for (int i = t; i < HG * DP; i += S::THREADS) qs[i] = i / DP < heads && i % DP < c.D ? q[i / DP * a.q_hs + i % DP] : 0.f;
+            __syncthreads();
+        } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (lane + 32 * e < c.D) o[e] = fmaf(w, to_f32(v[lane + 32 * e]), o[e] * f);
-            l = l * f + w;
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int h = nt * 8 + (lane >> 2), d = kk * 16 + i * 8 + (lane & 3) * 2;
+                        qf[nt][kk][i] = h < heads && d < c.D ? *reinterpret_cast<const uint32_t*>(q + h * a.q_hs + d) : 0u;
+                    }
+        }
+#pragma unroll
+        for (int i = 0; i < MC; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(acc) / 4); ++i) (&acc[0][0][0])[i] = 0.f;
+    };
+    begin();
+    int stage = 0, seg_chunk = cur.chunk;
+    bool seg_first = true;
+    int64_t flat = first;                                      // chunk in the row of all chunks
+
+    while (true) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();                                          // the tile is there, and the stage before is read
+        issue();
+        const int j = cur.chunk * CHUNK + warp * PT_KEYS, rows = cur.n - j;
+        float* sc_out = a.scores == nullptr ? nullptr : a.scores + (flat * CHUNK + warp * PT_KEYS) * a.rs;
+        if (rows > 0 && (live >> stage & 1)) {
+            const char* kt = tiles + stage * S::TILE;
+            const char* vt = kt + S::HALF;
+            if constexpr (!S::F32) {
+                const uint32_t row = saddr(kt) + (lane & 15) * S::ROW, sw = lane & 7, hi = lane >> 4;
+                float sc[2][NT][4];
+#pragma unroll
+                for (int i = 0; i < 8 * NT; ++i) (&sc[0][0][0])[i] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    uint32_t k4[4];
+                    ldsm4(row + (((kk * 2 + hi) ^ sw) << 4), k4);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(sc[kk & 1][nt], k4[0], k4[1], k4[2], k4[3], qf[nt][kk][0], qf[nt][kk][1], (const T*)nullptr);
+                }
+                uint32_t ph[NT][2], pl[NT][2];
+                bool moved = false;
+                float f[MC];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float s[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[e] = (sc[0][nt][e] + sc[1][nt][e]) * a.scale;
+                        if ((lane >> 2) + (e >> 1) * 8 >= rows) s[e] = -INFINITY;
+                    }
+                    if (sc_out != nullptr && nt * 8 + (lane & 3) * 2 < a.rs) {
+                        float* o = sc_out + (lane >> 2) * a.rs + nt * 8 + (lane & 3) * 2;
+                        if ((lane >> 2) < rows) __stcg(reinterpret_cast<float2*>(o), make_float2(s[0], s[1]));
+                        if ((lane >> 2) + 8 < rows) __stcg(reinterpret_cast<float2*>(o + 8 * a.rs), make_float2(s[2], s[3]));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int x = nt * 2 + i;
+                        float mx = fmaxf(s[i], s[i + 2]);
+                        mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 16));
+                        const float mn = fmaxf(m[x], mx);
+                        f[x] = pt_factor(m[x], mn);
+                        moved |= mn != m[x];
+                        m[x] = mn;
+                        s[i] = pt_factor(s[i], mn);
+                        s[i + 2] = pt_factor(s[i + 2], mn);
+                        l[x] = l[x] * f[x] + (s[i] + s[i + 2]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t h = pt_pack<T>(s[2 * i], s[2 * i + 1]);
+                        ph[nt][i] = pt_turn(h);
+                        pl[nt][i] = pt_turn(pt_pack<T>(s[2 * i] - pt_low<T>(h), s[2 * i + 1] - pt_high<T>(h)));
+                    }
+                }
+                if (__any_sync(FULL, moved)) {
+#pragma unroll
+                    for (int mt = 0; mt < KK; ++mt)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[mt][nt][e] *= f[nt * 2 + (e & 1)];
+                }
+                const uint32_t vrow = saddr(vt) + ((lane & 7) + (lane >> 4) * 8) * S::ROW;
+#pragma unroll
+                for (int mt = 0; mt < KK; ++mt) {
+                    uint32_t v4[4];
+                    ldsm4t(vrow + (((mt * 2 + (lane >> 3 & 1)) ^ sw) << 4), v4);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(acc[mt][nt], v4[0], v4[1], v4[2], v4[3], ph[nt][0], ph[nt][1], (const T*)nullptr);
+                        mma16816(acc[mt][nt], v4[0], v4[1], v4[2], v4[3], pl[nt][0], pl[nt][1], (const T*)nullptr);
+                    }
+                }
+            } else {
+                // scores: lane = key, each half of the warp one half of the head
+                const int key = lane & 15, half = lane >> 4;
+                float s[HG];
+#pragma unroll
+                for (int h = 0; h < HG; ++h) s[h] = 0.f;
+                const float4* kr = reinterpret_cast<const float4*>(kt + key * S::ROW);
+#pragma unroll 4
+                for (int i = 0; i < PIECES / 2; ++i) {
+                    const int p = half * (PIECES / 2) + i;
+                    const float4 k4 = kr[p ^ (key & 7)];
+#pragma unroll
+                    for (int h = 0; h < HG; ++h) {
+                        const float4 q4 = *reinterpret_cast<const float4*>(qs + h * DP + p * 4);
+                        s[h] = fmaf(k4.w, q4.w, fmaf(k4.z, q4.z, fmaf(k4.y, q4.y, fmaf(k4.x, q4.x, s[h]))));
+                    }
+                }
+                float f[HG];
+                bool moved = false;
+#pragma unroll
+                for (int h = 0; h < HG; ++h) {
+                    s[h] = (s[h] + __shfl_xor_sync(FULL, s[h], 16)) * a.scale;
+                    if (key >= rows) s[h] = -INFINITY;
+                    if (sc_out != nullptr && h < a.rs && key < rows && half == 0) __stcg(sc_out + key * a.rs + h, s[h]);
+                    float mx = s[h];
+#pragma unroll
+                    for (int o = 8; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+                    const float mn = fmaxf(m[h], mx);
+                    f[h] = pt_factor(m[h], mn);
+                    moved |= mn != m[h];
+                    m[h] = mn;
+                    s[h] = pt_factor(s[h], mn);
+                    l[h] = l[h] * f[h] + s[h];                 // both halves of the warp keep the same sums
+                    if (half == 0) ps[key * HG + h] = s[h];
+                }
+                __syncwarp();
+                if (moved) {
+#pragma unroll
+                    for (int h = 0; h < HG; ++h)
+#pragma unroll
+                        for (int i = 0; i < CPL; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[h][i][e] *= f[h];
+                }
+                constexpr int SPLIT = PIECES < 32 ? 32 / PIECES : 1;         // heads of 64: half a warp takes every second key
+#pragma unroll 4
+                for (int x = lane / (32 / SPLIT); x < PT_KEYS; x += SPLIT) {
+                    float w[HG];
+#pragma unroll
+                    for (int h = 0; h < HG; h += 4) load_vec<float, 4>(ps + x * HG + h, reinterpret_cast<float(&)[4]>(w[h]));
+#pragma unroll
+                    for (int i = 0; i < CPL; ++i) {
+                        const float4 v4 = reinterpret_cast<const float4*>(vt + x * S::ROW)[(lane % PIECES + i * 32) ^ (x & 7)];
+#pragma unroll
+                        for (int h = 0; h < HG; ++h) {
+                            acc[h][i][0] = fmaf(w[h], v4.x, acc[h][i][0]);
+                            acc[h][i][1] = fmaf(w[h], v4.y, acc[h][i][1]);
+                            acc[h][i][2] = fmaf(w[h], v4.z, acc[h][i][2]);
+                            acc[h][i][3] = fmaf(w[h], v4.w, acc[h][i][3]);
+                        }
+                    }
+                }
+                __syncwarp();                                  // the weights are read
+            }
+        } else if (sc_out != nullptr && rows > 0) {            // a page outside the pool: no weight
+            for (int i = lane; i < min(rows, PT_KEYS) * a.rs; i += 32) __stcg(sc_out + i, -INFINITY);
+        }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        --left;
+        ++flat;
+        if (cur.chunk + 1 < cur.chunks && left > 0) {
+            ++cur.chunk;
+            continue;
+        }
+        // ---- the block's warps join what they have of this pair
+#pragma unroll
+        for (int i = 0; i < MC; ++i) {
+            if constexpr (S::F32) {
+#pragma unroll
+                for (int o = 8; o >= 1; o >>= 1) l[i] += __shfl_xor_sync(FULL, l[i], o);
+                if (lane == 0) {
+                    ms[warp][i] = m[i];
+                    ls[warp][i] = l[i];
+                }
+            } else {
+                l[i] += __shfl_xor_sync(FULL, l[i], 4);
+                l[i] += __shfl_xor_sync(FULL, l[i], 8);
+                l[i] += __shfl_xor_sync(FULL, l[i], 16);
+                if (lane < 4) {
+                    ms[warp][i / 2 * 8 + lane * 2 + (i & 1)] = m[i];
+                    ls[warp][i / 2 * 8 + lane * 2 + (i & 1)] = l[i];
+                }
+            }
+        }
+        float* mine = os + warp * HG * OS;
+        if constexpr (S::F32) {
+#pragma unroll
+            for (int h = 0; h < HG; ++h)
+#pragma unroll
+                for (int i = 0; i < CPL; ++i) {
+                    float4 v = make_float4(acc[h][i][0], acc[h][i][1], acc[h][i][2], acc[h][i][3]);
+                    if constexpr (PIECES < 32) {
+                        v.x += __shfl_xor_sync(FULL, v.x, 16);
+                        v.y += __shfl_xor_sync(FULL, v.y, 16);
+                        v.z += __shfl_xor_sync(FULL, v.z, 16);
+                        v.w += __shfl_xor_sync(FULL, v.w, 16);
+                    }
+                    if (PIECES >= 32 || lane < PIECES) *reinterpret_cast<float4*>(mine + h * OS + (lane % PIECES + i * 32) * 4) = v;
+                }
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < KK; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mine[(nt * 8 + (lane & 3) * 2 + (e & 1)) * OS + mt * 16 + (lane >> 2) + (e >> 1) * 8] = acc[mt][nt][e];
+        }
+        __syncthreads();
+        const int g = cur.unit / a.groups, h0 = g * rep + cur.unit % a.groups * HG, heads = min(HG, (g + 1) * rep - h0);
+        const bool whole = seg_chunk == 0 && cur.chunk + 1 == cur.chunks;
+        float* part = whole ? nullptr : a.parts + ((int64_t)blockIdx.x * 2 + (seg_first ? 0 : 1)) * HG * (DP + 2);
+        for (int i = t; i < heads * (DP / 4); i += S::THREADS) {
+            const int h = i / (DP / 4), d = i % (DP / 4) * 4;
+            float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, ms[w][h]);
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = pt_factor(ms[w][h], mm);
+                const float4 x = *reinterpret_cast<const float4*>(os + (w * HG + h) * OS + d);
+                ll = fmaf(ls[w][h], f, ll);
+                o[0] = fmaf(x.x, f, o[0]);
+                o[1] = fmaf(x.y, f, o[1]);
+                o[2] = fmaf(x.z, f, o[2]);
+                o[3] = fmaf(x.w, f, o[3]);
+            }
+            if (whole) {
+                const float inv = pt_inverse(ll);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] *= inv;
+                if (d < c.D) store_vec<T, 4>((T*)a.out + cur.b * a.o_bs + (h0 + h) * a.o_hs + d, o);
+                if (d == 0 && a.stats != nullptr) *reinterpret_cast<float2*>(a.stats + ((int64_t)cur.b * a.H + h0 + h) * 2) = make_float2(mm, inv);
+            } else {
+                *reinterpret_cast<float4*>(part + h * DP + d) = make_float4(o[0], o[1], o[2], o[3]);
+                if (d == 0) *reinterpret_cast<float2*>(part + HG * DP + h * 2) = make_float2(mm, ll);
+            }
+        }
+        if (left == 0) break;
+        __syncthreads();                                       // sums are read
+        step(cur);
+        begin();
+        seg_chunk = 0;
+        seg_first = false;
+    }
+}
+
+// Where a pair's chunks stand, and which blocks' runs they are in
+struct PtSpan {
+    int64_t first, last, per;                                  // chunks of the row; chunks of a run
+    int chunks;
+};
+template <int CHUNK>
+__device__ __forceinline__ PtSpan pt_span(const sk_paged_cache& c, const PtArgs& a, int b, int unit, int blocks, int n, int64_t* red) {
+    int64_t total = 0, before = 0;
+    for (int i = threadIdx.x; i < c.B; i += blockDim.x) {
+        const int m = (paged_length(c, i, a.extra) + CHUNK - 1) / CHUNK;
+        total += m;
+        before += i < b ? m : 0;
+    }
+    const int units = c.G * a.groups;
+    PtSpan s;
+    s.per = (pt_block_sum(total, red) * units + blocks - 1) / blocks;
+    s.chunks = (n + CHUNK - 1) / CHUNK;
+    s.first = pt_block_sum(before, red) * units + (int64_t)unit * s.chunks;
+    s.last = s.first + s.chunks - 1;
+    return s;
+}
+// the partial result that block x left of a pair that begins at chunk `first`
+template <typename S> __device__ __forceinline__ const float* pt_part(const PtArgs& a, const PtSpan& s, int64_t x) {
+    return a.parts + (x * 2 + (s.first > x * s.per ? 1 : 0)) * S::HG * (S::DP + 2);
+}
+
+// The first B * H blocks join the partial results of a sequence and head, a warp every eighth one; the others add the weights of
+// PJ_KEYS keys of a sequence and key/value head to mass.
+constexpr int PJ_WARPS = 8, PJ_KEYS = 1024;
+template <typename S, typename T>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constant__ PtArgs a, int blocks) {
+    pdl_begin();
+    constexpr int DP = S::DP, HG = S::HG, E = DP / 32;
+    __shared__ int64_t red[PJ_WARPS];
+    __shared__ float ms[PJ_WARPS], ls[PJ_WARPS], os[PJ_WARPS][DP], stat[2][64];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, rep = a.H / c.G;
+    if (blockIdx.x < (unsigned)(c.B * a.H)) {
+        const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, unit = h / rep * a.groups + h % rep / HG, hh = h % rep % HG;
+        const int n = paged_length(c, b, a.extra);
+        if (n == 0) return;
+        const PtSpan s = pt_span<S::CHUNK>(c, a, b, unit, blocks, n, red);
+        const int64_t x0 = s.first / s.per, x1 = s.last / s.per;
+        if (x0 == x1) return;                                  // finished already
+        float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+        for (int64_t x = x0 + warp; x <= x1; x += PJ_WARPS) {
+            const float* part = pt_part<S>(a, s, x);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + HG * DP + hh * 2));
+            const float mn = fmaxf(m, ml.x), f = pt_factor(m, mn), fx = pt_factor(ml.x, mn);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(__ldcg(part + hh * DP + e * 32 + lane), fx, o[e] * f);
+            l = fmaf(ml.y, fx, l * f);
             m = mn;
         }
         if (lane == 0) {
@@ -55,44 +527,156 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const T* q, int64_t 
             ls[warp] = l;
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) os[warp][lane + 32 * e] = o[e];
+        for (int e = 0; e < E; ++e) os[warp][e * 32 + lane] = o[e];
         __syncthreads();
-        m = -INFINITY;
-        for (int w = 0; w < PT_WARPS; ++w) m = fmaxf(m, ms[w]);
-        const float mc = m == -INFINITY ? 0.f : m;
-        l = 0.f;
-        for (int w = 0; w < PT_WARPS; ++w) l += ls[w] * expf(ms[w] - mc);
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        for (int d = threadIdx.x; d < c.D; d += PT_WARPS * 32) {
-            float s = 0.f;
-            for (int w = 0; w < PT_WARPS; ++w) s += os[w][d] * expf(ms[w] - mc);
-            out[b * o_bs + h * o_hs + d] = from_f32<T>(s * inv);
-        }
-        if (c.mass != nullptr)
-            for (int j = warp; j < n; j += PT_WARPS) {
-                const int page = c.table[b * c.table_ld + (j >> shift)];
-                if (!paged_page_ok(c, page)) continue;
-                const float w = expf(score(j, page) - mc) * inv;
-                if (lane == 0) c.mass[b * c.mass_bs + g * c.mass_hs + j] += w;
+        if (t < c.D) {
+            m = -INFINITY;
+            l = 0.f;
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < PJ_WARPS; ++w) m = fmaxf(m, ms[w]);
+#pragma unroll
+            for (int w = 0; w < PJ_WARPS; ++w) {
+                const float f = pt_factor(ms[w], m);
+                l = fmaf(ls[w], f, l);
+                sum = fmaf(os[w][t], f, sum);
             }
+            ((T*)a.out)[b * a.o_bs + h * a.o_hs + t] = from_f32<T>(sum * pt_inverse(l));
+        }
+        return;
+    }
+    const unsigned x = blockIdx.x - c.B * a.H;
+    const int pieces = (c.width * c.page + PJ_KEYS - 1) / PJ_KEYS, j0 = (int)(x % pieces) * PJ_KEYS, g = x / pieces % c.G, b = x / pieces / c.G;
+    const int n = paged_length(c, b, a.extra);
+    if (j0 >= n) return;
+    const PtSpan s = pt_span<S::CHUNK>(c, a, b, g * a.groups, blocks, n, red);
+    float w[PJ_KEYS / (PJ_WARPS * 32)];
+#pragma unroll
+    for (int i = 0; i < PJ_KEYS / (PJ_WARPS * 32); ++i) w[i] = 0.f;
+    for (int grp = 0; grp < a.groups; ++grp) {
+        const int heads = min(HG, rep - grp * HG);
+        PtSpan u = s;
+        u.first += (int64_t)grp * s.chunks;
+        u.last += (int64_t)grp * s.chunks;
+        const int64_t x0 = u.first / u.per, x1 = u.last / u.per;
+        for (int h = warp; h < heads; h += PJ_WARPS) {         // final maximum and 1 / sum
+            float m = -INFINITY, l = 0.f;
+            if (x0 == x1) {
+                const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)b * a.H + g * rep + grp * HG + h) * 2));
+                m = st.x;
+                l = st.y;
+            } else {
+                for (int64_t x = x0 + lane; x <= x1; x += 32) {
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(pt_part<S>(a, u, x) + HG * DP + h * 2));
+                    const float mn = fmaxf(m, ml.x);
+                    l = l * pt_factor(m, mn) + ml.y * pt_factor(ml.x, mn);
+                    m = mn;
+                }
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) {
+                    const float m2 = __shfl_xor_sync(FULL, m, o), l2 = __shfl_xor_sync(FULL, l, o), mn = fmaxf(m, m2);
+                    l = l * pt_factor(m, mn) + l2 * pt_factor(m2, mn);
+                    m = mn;
+                }
+                l = pt_inverse(l);
+            }
+            if (lane == 0) {
+                stat[0][h] = m == -INFINITY ? 0.f : m;
+                stat[1][h] = l;
+            }
+        }
+        __syncthreads();
+        const float* sc = a.scores + u.first * S::CHUNK * a.rs;
+#pragma unroll
+        for (int i = 0; i < PJ_KEYS / (PJ_WARPS * 32); ++i) {
+            const int j = j0 + i * PJ_WARPS * 32 + t;
+            if (j < n)
+                for (int h = 0; h < heads; ++h) w[i] = fmaf(exp2_fast(__ldcg(sc + (int64_t)j * a.rs + h) - stat[0][h]), stat[1][h], w[i]);
+        }
         __syncthreads();
     }
+#pragma unroll
+    for (int i = 0; i < PJ_KEYS / (PJ_WARPS * 32); ++i) {
+        const int j = j0 + i * PJ_WARPS * 32 + t;
+        if (j < n) c.mass[b * c.mass_bs + g * c.mass_hs + j] += w[i];
+    }
+}
+
+struct PtPlan {
+    int groups, rs, chunk, blocks;
+    bool join;
+    size_t stats, scores, total;                               // bytes in front of them, and of all
+};
+template <typename S> PtPlan pt_plan(const sk_paged_cache& c, int H) {
+    PtPlan p;
+    const int rep = H / c.G;
+    p.groups = (rep + S::HG - 1) / S::HG;
+    p.rs = rep < S::HG ? (rep + 1) / 2 * 2 : S::HG;
+    const int64_t cap = (int64_t)c.width * c.page, chunks = (cap + S::CHUNK - 1) / S::CHUNK * c.B * c.G * p.groups;
+    const int64_t most = (int64_t)sm_count() * S::PER_SM;
+    p.blocks = (int)(chunks < most ? (chunks < 1 ? 1 : chunks) : most);
+    p.join = cap > S::CHUNK || c.mass != nullptr;
+    p.stats = cap > S::CHUNK ? up256((size_t)p.blocks * 2 * S::HG * (S::DP + 2) * 4) : 0;
+    p.scores = p.stats + (c.mass != nullptr ? up256((size_t)c.B * H * 8) : 0);
+    p.total = p.scores + (c.mass != nullptr ? up256((size_t)chunks * S::CHUNK * p.rs * 4) : 0);
+    return p;
+}
+
+// f(shape, element) of the kernel for this cache: heads padded to 64, 128 or 256; up to 8 (fp32: 4) query heads a block where a
+// key/value head has no more, else up to 16 (8): a key is read once for all of them.
+template <typename F> auto pt_with(const sk_paged_cache& c, int H, F&& f) {
+    auto sized = [&](auto t, auto nt) {
+        using T = decltype(t);
+        constexpr int NT = decltype(nt)::value;
+        if (c.D <= 64) return f(PtShape<T, 64, NT>{}, t);
+        if (c.D <= 128) return f(PtShape<T, 128, NT>{}, t);
+        return f(PtShape<T, 256, NT>{}, t);
+    };
+    auto typed = [&](auto t) {
+        if (H / c.G <= (sizeof(t) == 4 ? 4 : 8)) return sized(t, std::integral_constant<int, 1>{});
+        return sized(t, std::integral_constant<int, 2>{});
+    };
+    if (c.dtype == SK_F32) return typed(float{});
+    if (c.dtype == SK_BF16) return typed(__nv_bfloat16{});
+    return typed(__half{});
 }
 
 }  // namespace
 
-size_t paged_attn_workspace(const sk_paged_cache& c, int H) { return 0; }
+size_t paged_attn_workspace(const sk_paged_cache& c, int H) {
+    return pt_with(c, H, [&](auto s, auto) { return pt_plan<decltype(s)>(c, H).total; });
+}
 
 int launch_paged_attn(const sk_paged_cache& c, const void* q, int64_t q_bs, int64_t q_hs, void* out, int64_t o_bs, int64_t o_hs, int H,
                       int extra, float scale, void* workspace, cudaStream_t st) {
-    auto go = [&](auto t) {
+    return pt_with(c, H, [&](auto shape, auto t) -> int {
+        using S = decltype(shape);
         using T = decltype(t);
-        paged_attn_kernel<T><<<c.B * c.G, PT_WARPS * 32, 0, st>>>(c, (const T*)q, q_bs, q_hs, (T*)out, o_bs, o_hs, H, extra, scale);
-    };
-    if (c.dtype == SK_F32) go(float{});
-    else if (c.dtype == SK_BF16) go(__nv_bfloat16{});
-    else go(__half{});
-    return check_launch("paged_attn_kernel");
+        const PtPlan p = pt_plan<S>(c, H);
+        const int64_t pieces = ((int64_t)c.width * c.page + PJ_KEYS - 1) / PJ_KEYS;
+        const int64_t joins = (int64_t)c.B * H + (c.mass != nullptr ? pieces * c.B * c.G : 0);
+        if (joins > INT32_MAX) return fail(SK_ERR_UNSUPPORTED, "sk_paged_attn: %d sequences of up to %lld keys", c.B, (long long)c.width * c.page);
+        PtArgs a;
+        a.q = q;
+        a.out = out;
+        a.parts = (float*)workspace;
+        a.stats = c.mass != nullptr ? (float*)((char*)workspace + p.stats) : nullptr;
+        a.scores = c.mass != nullptr ? (float*)((char*)workspace + p.scores) : nullptr;
+        a.q_bs = q_bs;
+        a.q_hs = q_hs;
+        a.o_bs = o_bs;
+        a.o_hs = o_hs;
+        a.H = H;
+        a.extra = extra;
+        a.groups = p.groups;
+        a.rs = p.rs;
+        a.scale = scale * PT_LOG2E;
+        cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<S, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        if (e == cudaSuccess) e = launch_after(paged_attn_kernel<S, T>, dim3(p.blocks), dim3(S::THREADS), S::SMEM, st, c, a);
+        if (int rc = check_chained(e, "paged_attn_kernel")) return rc;
+        if (!p.join) return SK_OK;
+        return check_chained(launch_after(paged_join_kernel<S, T>, dim3((unsigned)joins), dim3(PJ_WARPS * 32), 0, st, c, a, p.blocks), "paged_join_kernel");
+    });
 }
 
 }  // namespace sk
