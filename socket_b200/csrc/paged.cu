@@ -65,6 +65,8 @@ int paged_check(const sk_paged_cache* c, const char* what) {
     if (c->D % v != 0 || c->D > 256) return fail(SK_ERR_UNSUPPORTED, "%s: head size %d", what, c->D);
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->k_ps % v || c->k_hs % v || c->k_rs % v || c->v_ps % v || c->v_hs % v || c->v_rs % v)
         return fail(SK_ERR_MISALIGNED, "%s: pools and their strides must be 16-byte aligned", what);
+    // the offset of a page's row is a product of 32-bit numbers
+    if (c->k_rs < 0 || c->v_rs < 0 || c->k_rs > INT32_MAX / 4 || c->v_rs > INT32_MAX / 4) return fail(SK_ERR_UNSUPPORTED, "%s: row strides", what);
     return SK_OK;
 }
 

@@ -22,6 +22,9 @@ namespace {
 
 constexpr float PT_LOG2E = 1.4426950408889634f;
 constexpr int PT_KEYS = 16;                                    // keys of a warp's tile
+// A running maximum is only raised for a score this far (in powers of two) above it: weights then reach 2^8, which neither a half nor
+// the sums mind, and the six exchanges and the rescaling that a rise takes are left out of nearly every tile.
+constexpr float PT_SLACK = 8.f;
 
 template <typename T, int DP_, int NT_> struct PtShape {
     static constexpr int DP = DP_, NT = NT_;                   // head size padded, groups of heads
@@ -32,13 +35,21 @@ template <typename T, int DP_, int NT_> struct PtShape {
     static constexpr int CHUNK = WARPS * PT_KEYS, THREADS = WARPS * 32;
     static constexpr int OS = DP + 4;                          // row of the joined sums: columns of four query pairs in four bank groups
     static constexpr size_t SMEM = (size_t)WARPS * STAGES * TILE + (size_t)WARPS * HG * OS * 4 + (F32 ? (size_t)HG * DP * 4 + (size_t)WARPS * PT_KEYS * HG * 4 : 0);
-    static constexpr int PER_SM = SMEM <= 112 * 1024 ? 2 : 1;
+    static constexpr int PER_SM = SMEM <= 113 * 1024 ? 2 : 1;
     static_assert(SMEM <= 226 * 1024, "shared memory of a block");
+};
+
+// What the second kernel has to know of a block's run: where it begins, how long it is, the chunks of every run; and the pair that begins
+// in it and ends in a later run, `tail_last` (-1: none)
+struct alignas(16) PtRun {
+    int64_t per, first;                                        // chunks of a run, and before this one
+    int b, g, grp, chunk, chunks, n, left, tail_last, tail_b, tail_g, tail_grp, tail_inside;
 };
 
 struct PtArgs {
     const void* q;
     void* out;
+    PtRun* runs;
     float *parts, *stats, *scores;                             // partial results; final maximum and 1 / sum per head; scores for mass
     int64_t q_bs, q_hs, o_bs, o_hs;
     int H, extra, groups, rs;                                  // groups of HG heads per key/value head; scores of a key
@@ -82,10 +93,27 @@ template <> __device__ __forceinline__ float pt_high<__half>(uint32_t x) { retur
 __device__ __forceinline__ float pt_factor(float a, float b) { return exp2_fast(a - (b == -INFINITY ? 0.f : b)); }
 __device__ __forceinline__ float pt_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-// A place in the row of chunks: chunk `chunk` of `chunks` of pair `unit` of sequence b, which has n keys
+// A place in the row of chunks: chunk `chunk` of `chunks` of group grp of key/value head g of sequence b, which has n keys.  Behind the
+// chunks of every group stand PT_PAD empty ones: what it costs a block to finish it and begin the next.
+constexpr int PT_PAD = 1;
 struct PtPlace {
-    int b, unit, chunk, chunks, n;
+    int b, g, grp, chunk, chunks, n;
 };
+// to the next chunk, with what is left of the run; past the end of the run nothing is read
+template <int CHUNK> __device__ __forceinline__ void pt_step(const sk_paged_cache& c, const PtArgs& a, PtPlace& p, int& left) {
+    --left;
+    if (++p.chunk < p.chunks) return;
+    left -= PT_PAD;
+    p.chunk = 0;
+    if (left <= 0 || ++p.grp < a.groups) return;
+    p.grp = 0;
+    if (++p.g < c.G) return;
+    p.g = 0;
+    do {
+        p.n = ++p.b < c.B ? paged_length(c, p.b, a.extra) : 1;
+    } while (p.n == 0);
+    p.chunks = (p.n + CHUNK - 1) / CHUNK;
+}
 
 template <typename S, typename T>
 __global__ void __launch_bounds__(S::THREADS, S::PER_SM)
@@ -101,13 +129,13 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
     float* os = reinterpret_cast<float*>(pt_smem + WARPS * STAGES * S::TILE);                       // [WARPS][HG][OS]
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, shift = 31 - __clz(c.page);
     const int units = c.G * a.groups, rep = a.H / c.G;
-    auto chunks_of = [](int n) { return (n + CHUNK - 1) / CHUNK; };
+    auto slots_of = [](int n) { return n == 0 ? 0 : (n + CHUNK - 1) / CHUNK + PT_PAD; };
 
     // ---- this block's run of chunks
     int64_t total = 0;
     for (int b = t; b < c.B; b += S::THREADS) {
         bool over;
-        total += chunks_of(paged_length(c, b, a.extra, &over));
+        total += slots_of(paged_length(c, b, a.extra, &over));
         if (over && blockIdx.x == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
     }
     total = pt_block_sum(total, red) * units;
@@ -116,10 +144,15 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
             for (int i = t; i < a.H * c.D; i += S::THREADS) ((T*)a.out)[b * a.o_bs + i / c.D * a.o_hs + i % c.D] = from_f32<T>(0.f);
     const int64_t per = (total + gridDim.x - 1) / gridDim.x, first = per * blockIdx.x;
     int left = (int)max(min(per, total - first), (int64_t)0);
+    PtRun* run = a.runs == nullptr ? nullptr : a.runs + blockIdx.x;
+    if (run != nullptr && t == 0) {
+        run->left = 0;
+        run->tail_last = -1;
+    }
     if (left == 0) return;
     int64_t before = 0;
     for (int b0 = 0; b0 < c.B; b0 += S::THREADS) {             // the sequence that holds chunk `first`
-        const int b = b0 + t, n = b < c.B ? paged_length(c, b, a.extra) : 0, m = chunks_of(n);
+        const int b = b0 + t, n = b < c.B ? paged_length(c, b, a.extra) : 0, m = slots_of(n);
         int64_t sum = m;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -134,24 +167,32 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
             all += red[w];
         }
         const int64_t lo = (before + sum - m) * units, hi = (before + sum) * units;
-        if (lo <= first && first < hi) start_s = PtPlace{b, (int)((first - lo) / m), (int)((first - lo) % m), m, n};
+        if (lo <= first && first < hi) {
+            const int unit = (int)((first - lo) / m);
+            start_s = PtPlace{b, unit / a.groups, unit % a.groups, (int)((first - lo) % m), m - PT_PAD, n};
+        }
         before += all;
         __syncthreads();
         if (before * units > first) break;
     }
-    PtPlace cur = start_s, ld = cur;
-    auto step = [&](PtPlace& p) {
-        if (++p.chunk < p.chunks) return;
-        p.chunk = 0;
-        if (++p.unit < units) return;
-        p.unit = 0;
-        do {
-            p.n = ++p.b < c.B ? paged_length(c, p.b, a.extra) : 1;
-        } while (p.n == 0);
-        p.chunks = chunks_of(p.n);
-    };
+    PtPlace cur = start_s;
+    int64_t flat = first;                                      // chunk in the row of all chunks
+    if (cur.chunk >= cur.chunks) {                             // the run begins behind a pair
+        const int skip = cur.chunks + PT_PAD - cur.chunk;
+        cur.chunk = cur.chunks - 1;
+        left += 1 + PT_PAD - skip;
+        flat += skip;
+        pt_step<CHUNK>(c, a, cur, left);
+        if (left <= 0) return;
+    }
+    PtPlace ld = cur;
+    if (run != nullptr && t == 0) *run = PtRun{per, flat, cur.b, cur.g, cur.grp, cur.chunk, cur.chunks, cur.n, left, -1, 0, 0, 0, 0};
 
     // ---- copies: this warp's tile of the chunk at `ld`, one commit group each; `live` has a bit per stage that holds keys
+    constexpr int COPIES = PT_KEYS * PIECES / 32;              // of keys, and of values, per lane
+    const int k_row = (int)c.k_rs * (int)sizeof(T), v_row = (int)c.v_rs * (int)sizeof(T);          // bytes; checked to fit
+    const char *k_head = (const char*)c.k + ld.g * c.k_hs * (int)sizeof(T), *v_head = (const char*)c.v + ld.g * c.v_hs * (int)sizeof(T);
+    const uint32_t ld_to = lane / PIECES * S::ROW + ((lane % PIECES ^ (lane / PIECES & 7)) << 4);
     int ld_left = left, ld_stage = 0, ld_page = 0;
     uint32_t live = 0;
     auto ask_page = [&]() {
@@ -164,25 +205,40 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
             const int j = ld.chunk * CHUNK + warp * PT_KEYS, rows = ld.n - j;
             if (rows > 0) {
                 if (paged_page_ok(c, ld_page)) {
-                    const int g = ld.unit / a.groups;
-                    const T* k = (const T*)c.k + ld_page * c.k_ps + g * c.k_hs + (j & (c.page - 1)) * c.k_rs;
-                    const T* v = (const T*)c.v + ld_page * c.v_ps + g * c.v_hs + (j & (c.page - 1)) * c.v_rs;
+                    const char* k = k_head + ld_page * (c.k_ps * (int)sizeof(T)) + (int64_t)(j & (c.page - 1)) * k_row;
+                    const char* v = v_head + ld_page * (c.v_ps * (int)sizeof(T)) + (int64_t)(j & (c.page - 1)) * v_row;
                     const uint32_t dst = saddr(tiles + ld_stage * S::TILE);
+                    if (rows >= PT_KEYS && c.D == DP) {
+                        const char* kl = k + (int64_t)(lane / PIECES) * k_row + lane % PIECES * 16;
+                        const char* vl = v + (int64_t)(lane / PIECES) * v_row + lane % PIECES * 16;
 #pragma unroll
-                    for (int i = 0; i < PT_KEYS * PIECES / 32; ++i) {
-                        const int x = i * 32 + lane, r = x / PIECES, p = x % PIECES;
-                        const bool in = r < rows && p * VE < c.D;      // others are zeros
-                        const uint32_t at = dst + r * S::ROW + ((p ^ (r & 7)) << 4);
-                        cp16(at, in ? k + r * c.k_rs + p * VE : k, in);
-                        cp16(at + S::HALF, in ? v + r * c.v_rs + p * VE : v, in);
+                        for (int i = 0; i < COPIES; ++i) {
+                            const int r = i * 32 / PIECES;     // of lane 0; lanes add at most bits that r has clear
+                            const uint32_t at = (dst + ld_to) ^ ((r & 7) << 4);
+                            cp16(at + r * S::ROW + i * 32 % PIECES * 16, kl + (int64_t)r * k_row + i * 32 % PIECES * 16, true);
+                            cp16(at + r * S::ROW + i * 32 % PIECES * 16 + S::HALF, vl + (int64_t)r * v_row + i * 32 % PIECES * 16, true);
+                        }
+                    } else {
+#pragma unroll 2
+                        for (int i = 0; i < COPIES; ++i) {
+                            const int x = i * 32 + lane, r = x / PIECES, p = x % PIECES;
+                            const bool in = r < rows && p * VE < c.D;      // others are zeros
+                            const uint32_t at = dst + r * S::ROW + ((p ^ (r & 7)) << 4);
+                            cp16(at, in ? k + (int64_t)r * k_row + p * 16 : k, in);
+                            cp16(at + S::HALF, in ? v + (int64_t)r * v_row + p * 16 : v, in);
+                        }
                     }
                     live |= 1u << ld_stage;
                 } else if (lane == 0 && c.status != nullptr) {
                     atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
                 }
             }
-            --ld_left;
-            if (ld_left > 0) step(ld);
+            const int g = ld.g;
+            pt_step<CHUNK>(c, a, ld, ld_left);
+            if (ld.g != g) {
+                k_head = (const char*)c.k + ld.g * c.k_hs * (int)sizeof(T);
+                v_head = (const char*)c.v + ld.g * c.v_hs * (int)sizeof(T);
+            }
             ask_page();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -200,12 +256,11 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
     float m[MC], l[MC];
     float* qs = os + WARPS * HG * OS;                          // fp32: [HG][DP] queries, [WARPS][16][HG] weights
     float* ps = qs + HG * DP + warp * PT_KEYS * HG;
-    auto begin = [&]() {
-        const int g = cur.unit / a.groups, h0 = g * rep + cur.unit % a.groups * HG, heads = min(HG, (g + 1) * rep - h0);
-        const T* q = (const T*)a.q + cur.b * a.q_bs + h0 * a.q_hs;
+    auto queries = [&](const PtPlace& p) {
+        const int h0 = p.g * rep + p.grp * HG, heads = min(HG, (p.g + 1) * rep - h0);
+        const T* q = (const T*)a.q + p.b * a.q_bs + h0 * a.q_hs;
         if constexpr (S::F32) {
             for (int i = t; i < HG * DP; i += S::THREADS) qs[i] = i / DP < heads && i % DP < c.D ? q[i / DP * a.q_hs + i % DP] : 0.f;
-            __syncthreads();
         } else {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -217,6 +272,8 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                         qf[nt][kk][i] = h < heads && d < c.D ? *reinterpret_cast<const uint32_t*>(q + h * a.q_hs + d) : 0u;
                     }
         }
+    };
+    auto begin = [&]() {
 #pragma unroll
         for (int i = 0; i < MC; ++i) {
             m[i] = -INFINITY;
@@ -225,10 +282,11 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(acc) / 4); ++i) (&acc[0][0][0])[i] = 0.f;
     };
+    queries(cur);
+    if (S::F32) __syncthreads();
     begin();
     int stage = 0, seg_chunk = cur.chunk;
-    bool seg_first = true;
-    int64_t flat = first;                                      // chunk in the row of all chunks
+    bool seg_first = flat == first;                            // what the run begins with, inside a pair or with it
 
     while (true) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
@@ -240,68 +298,80 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
             const char* kt = tiles + stage * S::TILE;
             const char* vt = kt + S::HALF;
             if constexpr (!S::F32) {
-                const uint32_t row = saddr(kt) + (lane & 15) * S::ROW, sw = lane & 7, hi = lane >> 4;
+                // 16-byte piece p of row r lies at piece p ^ (r & 7): of two pieces a step, the step's bits are flipped in the address
+                const uint32_t row = saddr(kt) + (lane & 15) * S::ROW + (((lane >> 4) ^ (lane & 7)) << 4);
                 float sc[2][NT][4];
 #pragma unroll
                 for (int i = 0; i < 8 * NT; ++i) (&sc[0][0][0])[i] = 0.f;
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
                     uint32_t k4[4];
-                    ldsm4(row + (((kk * 2 + hi) ^ sw) << 4), k4);
+                    ldsm4(row ^ (kk << 5), k4);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(sc[kk & 1][nt], k4[0], k4[1], k4[2], k4[3], qf[nt][kk][0], qf[nt][kk][1], (const T*)nullptr);
                 }
-                uint32_t ph[NT][2], pl[NT][2];
-                bool moved = false;
-                float f[MC];
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][e] = (sc[0][nt][e] + sc[1][nt][e]) * a.scale;
+                if (rows < PT_KEYS) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if ((lane >> 2) + (e >> 1) * 8 >= rows) s[nt][e] = -INFINITY;
+                }
+                bool above = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float s[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[e] = (sc[0][nt][e] + sc[1][nt][e]) * a.scale;
-                        if ((lane >> 2) + (e >> 1) * 8 >= rows) s[e] = -INFINITY;
-                    }
                     if (sc_out != nullptr && nt * 8 + (lane & 3) * 2 < a.rs) {
                         float* o = sc_out + (lane >> 2) * a.rs + nt * 8 + (lane & 3) * 2;
-                        if ((lane >> 2) < rows) __stcg(reinterpret_cast<float2*>(o), make_float2(s[0], s[1]));
-                        if ((lane >> 2) + 8 < rows) __stcg(reinterpret_cast<float2*>(o + 8 * a.rs), make_float2(s[2], s[3]));
+                        if ((lane >> 2) < rows) __stcg(reinterpret_cast<float2*>(o), make_float2(s[nt][0], s[nt][1]));
+                        if ((lane >> 2) + 8 < rows) __stcg(reinterpret_cast<float2*>(o + 8 * a.rs), make_float2(s[nt][2], s[nt][3]));
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int x = nt * 2 + i;
-                        float mx = fmaxf(s[i], s[i + 2]);
+                    for (int i = 0; i < 2; ++i) above |= fmaxf(s[nt][i], s[nt][i + 2]) > m[nt * 2 + i] + PT_SLACK;
+                }
+                if (__any_sync(FULL, above)) {                 // maxima follow, and what was summed up with them
+#pragma unroll
+                    for (int x = 0; x < MC; ++x) {
+                        float mx = fmaxf(s[x / 2][x & 1], s[x / 2][(x & 1) + 2]);
                         mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 16));
-                        const float mn = fmaxf(m[x], mx);
-                        f[x] = pt_factor(m[x], mn);
-                        moved |= mn != m[x];
+                        const float mn = fmaxf(m[x], mx), f = pt_factor(m[x], mn);
                         m[x] = mn;
-                        s[i] = pt_factor(s[i], mn);
-                        s[i + 2] = pt_factor(s[i + 2], mn);
-                        l[x] = l[x] * f[x] + (s[i] + s[i + 2]);
+                        l[x] *= f;
+#pragma unroll
+                        for (int mt = 0; mt < KK; ++mt) {
+                            acc[mt][x / 2][x & 1] *= f;
+                            acc[mt][x / 2][(x & 1) + 2] *= f;
+                        }
+                    }
+                }
+                uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float mc = m[nt * 2 + i] == -INFINITY ? 0.f : m[nt * 2 + i];
+                        s[nt][i] = exp2_fast(s[nt][i] - mc);
+                        s[nt][i + 2] = exp2_fast(s[nt][i + 2] - mc);
+                        l[nt * 2 + i] += s[nt][i] + s[nt][i + 2];
                     }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t h = pt_pack<T>(s[2 * i], s[2 * i + 1]);
+                        const uint32_t h = pt_pack<T>(s[nt][2 * i], s[nt][2 * i + 1]);
                         ph[nt][i] = pt_turn(h);
-                        pl[nt][i] = pt_turn(pt_pack<T>(s[2 * i] - pt_low<T>(h), s[2 * i + 1] - pt_high<T>(h)));
+                        pl[nt][i] = pt_turn(pt_pack<T>(s[nt][2 * i] - pt_low<T>(h), s[nt][2 * i + 1] - pt_high<T>(h)));
                     }
                 }
-                if (__any_sync(FULL, moved)) {
-#pragma unroll
-                    for (int mt = 0; mt < KK; ++mt)
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[mt][nt][e] *= f[nt * 2 + (e & 1)];
-                }
-                const uint32_t vrow = saddr(vt) + ((lane & 7) + (lane >> 4) * 8) * S::ROW;
+                const uint32_t vrow = saddr(vt) + ((lane & 7) + (lane >> 4) * 8) * S::ROW + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
 #pragma unroll
                 for (int mt = 0; mt < KK; ++mt) {
                     uint32_t v4[4];
-                    ldsm4t(vrow + (((mt * 2 + (lane >> 3 & 1)) ^ sw) << 4), v4);
+                    ldsm4t(vrow ^ (mt << 5), v4);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         mma16816(acc[mt][nt], v4[0], v4[1], v4[2], v4[3], ph[nt][0], ph[nt][1], (const T*)nullptr);
@@ -325,33 +395,36 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                         s[h] = fmaf(k4.w, q4.w, fmaf(k4.z, q4.z, fmaf(k4.y, q4.y, fmaf(k4.x, q4.x, s[h]))));
                     }
                 }
-                float f[HG];
-                bool moved = false;
+                bool above = false;
 #pragma unroll
                 for (int h = 0; h < HG; ++h) {
                     s[h] = (s[h] + __shfl_xor_sync(FULL, s[h], 16)) * a.scale;
                     if (key >= rows) s[h] = -INFINITY;
                     if (sc_out != nullptr && h < a.rs && key < rows && half == 0) __stcg(sc_out + key * a.rs + h, s[h]);
-                    float mx = s[h];
-#pragma unroll
-                    for (int o = 8; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
-                    const float mn = fmaxf(m[h], mx);
-                    f[h] = pt_factor(m[h], mn);
-                    moved |= mn != m[h];
-                    m[h] = mn;
-                    s[h] = pt_factor(s[h], mn);
-                    l[h] = l[h] * f[h] + s[h];                 // both halves of the warp keep the same sums
-                    if (half == 0) ps[key * HG + h] = s[h];
+                    above |= s[h] > m[h] + PT_SLACK;
                 }
-                __syncwarp();
-                if (moved) {
+                if (__any_sync(FULL, above)) {
 #pragma unroll
-                    for (int h = 0; h < HG; ++h)
+                    for (int h = 0; h < HG; ++h) {
+                        float mx = s[h];
+#pragma unroll
+                        for (int o = 8; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+                        const float mn = fmaxf(m[h], mx), f = pt_factor(m[h], mn);
+                        m[h] = mn;
+                        l[h] *= f;
 #pragma unroll
                         for (int i = 0; i < CPL; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[h][i][e] *= f[h];
+                            for (int e = 0; e < 4; ++e) acc[h][i][e] *= f;
+                    }
                 }
+#pragma unroll
+                for (int h = 0; h < HG; ++h) {
+                    const float w = pt_factor(s[h], m[h]);
+                    l[h] += w;                                 // both halves of the warp keep the same sums
+                    if (half == 0) ps[key * HG + h] = w;
+                }
+                __syncwarp();
                 constexpr int SPLIT = PIECES < 32 ? 32 / PIECES : 1;         // heads of 64: half a warp takes every second key
 #pragma unroll 4
                 for (int x = lane / (32 / SPLIT); x < PT_KEYS; x += SPLIT) {
@@ -376,13 +449,17 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
             for (int i = lane; i < min(rows, PT_KEYS) * a.rs; i += 32) __stcg(sc_out + i, -INFINITY);
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        --left;
-        ++flat;
-        if (cur.chunk + 1 < cur.chunks && left > 0) {
+        if (cur.chunk + 1 < cur.chunks && left > 1) {
+            --left;
+            ++flat;
             ++cur.chunk;
             continue;
         }
-        // ---- the block's warps join what they have of this pair
+        // ---- the block's warps join what they have of this pair; the next one's queries are on their way meanwhile
+        PtPlace next = cur;
+        pt_step<CHUNK>(c, a, next, left);
+        if (!S::F32 && left > 0) queries(next);
+        const int tiles_here = (min(cur.n, (cur.chunk + 1) * CHUNK) - seg_chunk * CHUNK + PT_KEYS - 1) / PT_KEYS, busy = min(tiles_here, WARPS);
 #pragma unroll
         for (int i = 0; i < MC; ++i) {
             if constexpr (S::F32) {
@@ -424,10 +501,10 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        mine[(nt * 8 + (lane & 3) * 2 + (e & 1)) * OS + mt * 16 + (lane >> 2) + (e >> 1) * 8] = acc[mt][nt][e];
+                        if (warp < busy && nt * 8 + (lane & 3) * 2 < rep) mine[(nt * 8 + (lane & 3) * 2 + (e & 1)) * OS + mt * 16 + (lane >> 2) + (e >> 1) * 8] = acc[mt][nt][e];
         }
         __syncthreads();
-        const int g = cur.unit / a.groups, h0 = g * rep + cur.unit % a.groups * HG, heads = min(HG, (g + 1) * rep - h0);
+        const int h0 = cur.g * rep + cur.grp * HG, heads = min(HG, (cur.g + 1) * rep - h0);
         const bool whole = seg_chunk == 0 && cur.chunk + 1 == cur.chunks;
         float* part = whole ? nullptr : a.parts + ((int64_t)blockIdx.x * 2 + (seg_first ? 0 : 1)) * HG * (DP + 2);
         for (int i = t; i < heads * (DP / 4); i += S::THREADS) {
@@ -436,8 +513,7 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, ms[w][h]);
             float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
+            for (int w = 0; w < busy; ++w) {                   // the others had no key of it
                 const float f = pt_factor(ms[w][h], mm);
                 const float4 x = *reinterpret_cast<const float4*>(os + (w * HG + h) * OS + d);
                 ll = fmaf(ls[w][h], f, ll);
@@ -457,68 +533,58 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                 if (d == 0) *reinterpret_cast<float2*>(part + HG * DP + h * 2) = make_float2(mm, ll);
             }
         }
-        if (left == 0) break;
+        if (left <= 0) break;
         __syncthreads();                                       // sums are read
-        step(cur);
+        flat += 1 + PT_PAD;
+        cur = next;
+        if (S::F32) {
+            queries(cur);
+            __syncthreads();
+        }
         begin();
         seg_chunk = 0;
         seg_first = false;
     }
-}
-
-// Where a pair's chunks stand, and which blocks' runs they are in
-struct PtSpan {
-    int64_t first, last, per;                                  // chunks of the row; chunks of a run
-    int chunks;
-};
-template <int CHUNK>
-__device__ __forceinline__ PtSpan pt_span(const sk_paged_cache& c, const PtArgs& a, int b, int unit, int blocks, int n, int64_t* red) {
-    int64_t total = 0, before = 0;
-    for (int i = threadIdx.x; i < c.B; i += blockDim.x) {
-        const int m = (paged_length(c, i, a.extra) + CHUNK - 1) / CHUNK;
-        total += m;
-        before += i < b ? m : 0;
+    if (run != nullptr && t == 0 && seg_chunk == 0 && cur.chunk + 1 < cur.chunks) {
+        run->tail_b = cur.b;
+        run->tail_g = cur.g;
+        run->tail_grp = cur.grp;
+        run->tail_inside = !seg_first;
+        run->tail_last = (int)((flat - cur.chunk + cur.chunks - 1) / per);
     }
-    const int units = c.G * a.groups;
-    PtSpan s;
-    s.per = (pt_block_sum(total, red) * units + blocks - 1) / blocks;
-    s.chunks = (n + CHUNK - 1) / CHUNK;
-    s.first = pt_block_sum(before, red) * units + (int64_t)unit * s.chunks;
-    s.last = s.first + s.chunks - 1;
-    return s;
-}
-// the partial result that block x left of a pair that begins at chunk `first`
-template <typename S> __device__ __forceinline__ const float* pt_part(const PtArgs& a, const PtSpan& s, int64_t x) {
-    return a.parts + (x * 2 + (s.first > x * s.per ? 1 : 0)) * S::HG * (S::DP + 2);
 }
 
-// The first B * H blocks join the partial results of a sequence and head, a warp every eighth one; the others add the weights of
-// PJ_KEYS keys of a sequence and key/value head to mass.
-constexpr int PJ_WARPS = 8, PJ_KEYS = 1024;
+// The partial result that block x left of a pair: its run's first one, or, of a pair that begins inside the run, its last one
+template <typename S> __device__ __forceinline__ const float* pt_part(const PtArgs& a, int x, bool begins_inside) {
+    return a.parts + ((int64_t)x * 2 + (begins_inside ? 1 : 0)) * S::HG * (S::DP + 2);
+}
+
+// A pair that ends in another run than it begins in belongs to the run it begins in; a run has one such pair at most.  The first HG
+// blocks of a run (blockIdx.x) join its partial results, one head each, a warp every eighth of them; the others, with mass, add the
+// weights of a share of the run's keys.
+constexpr int PJ_WARPS = 8, PJ_SHARES = 4;
 template <typename S, typename T>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
-paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constant__ PtArgs a, int blocks) {
+paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constant__ PtArgs a) {
     pdl_begin();
-    constexpr int DP = S::DP, HG = S::HG, E = DP / 32;
-    __shared__ int64_t red[PJ_WARPS];
-    __shared__ float ms[PJ_WARPS], ls[PJ_WARPS], os[PJ_WARPS][DP], stat[2][64];
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, rep = a.H / c.G;
-    if (blockIdx.x < (unsigned)(c.B * a.H)) {
-        const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, unit = h / rep * a.groups + h % rep / HG, hh = h % rep % HG;
-        const int n = paged_length(c, b, a.extra);
-        if (n == 0) return;
-        const PtSpan s = pt_span<S::CHUNK>(c, a, b, unit, blocks, n, red);
-        const int64_t x0 = s.first / s.per, x1 = s.last / s.per;
-        if (x0 == x1) return;                                  // finished already
+    constexpr int DP = S::DP, HG = S::HG, E = DP / 32, CHUNK = S::CHUNK;
+    __shared__ float ms[PJ_WARPS], ls[PJ_WARPS], os[PJ_WARPS][DP], stat[2][HG];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, rep = a.H / c.G, x0 = blockIdx.x;
+    PtRun run;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(PtRun) / 16); ++i) reinterpret_cast<int4*>(&run)[i] = __ldcg(reinterpret_cast<const int4*>(a.runs + x0) + i);
+    if (blockIdx.y < HG) {
+        const int last = run.tail_last, h = blockIdx.y, b = run.tail_b, g = run.tail_g, hh = run.tail_grp * HG + h;
+        if (last < 0 || hh >= rep) return;
         float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.f;
-        for (int64_t x = x0 + warp; x <= x1; x += PJ_WARPS) {
-            const float* part = pt_part<S>(a, s, x);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + HG * DP + hh * 2));
+        for (int x = x0 + warp; x <= last; x += PJ_WARPS) {
+            const float* part = pt_part<S>(a, x, x == x0 && run.tail_inside);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + HG * DP + h * 2));
             const float mn = fmaxf(m, ml.x), f = pt_factor(m, mn), fx = pt_factor(ml.x, mn);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(__ldcg(part + hh * DP + e * 32 + lane), fx, o[e] * f);
+            for (int e = 0; e < E; ++e) o[e] = fmaf(__ldcg(part + h * DP + e * 32 + lane), fx, o[e] * f);
             l = fmaf(ml.y, fx, l * f);
             m = mn;
         }
@@ -541,82 +607,102 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                 l = fmaf(ls[w], f, l);
                 sum = fmaf(os[w][t], f, sum);
             }
-            ((T*)a.out)[b * a.o_bs + h * a.o_hs + t] = from_f32<T>(sum * pt_inverse(l));
+            ((T*)a.out)[b * a.o_bs + (g * rep + hh) * a.o_hs + t] = from_f32<T>(sum * pt_inverse(l));
         }
         return;
     }
-    const unsigned x = blockIdx.x - c.B * a.H;
-    const int pieces = (c.width * c.page + PJ_KEYS - 1) / PJ_KEYS, j0 = (int)(x % pieces) * PJ_KEYS, g = x / pieces % c.G, b = x / pieces / c.G;
-    const int n = paged_length(c, b, a.extra);
-    if (j0 >= n) return;
-    const PtSpan s = pt_span<S::CHUNK>(c, a, b, g * a.groups, blocks, n, red);
-    float w[PJ_KEYS / (PJ_WARPS * 32)];
+    // ---- mass: pairs and heads of one key/value head add to the same keys; a block adds what all heads of a group weigh, so more
+    // than one group takes turns: units of a key/value head stand one behind the other, and only the first one's chunks are walked
+    const int share = blockIdx.y - HG, from = (int)((int64_t)run.left * share / PJ_SHARES), to = (int)((int64_t)run.left * (share + 1) / PJ_SHARES);
+    const int64_t per = run.per;
+    PtPlace p = {run.b, run.g, run.grp, run.chunk, run.chunks, run.n};
+    int64_t flat = run.first;
+    for (int done = 0; done < to;) {
+        const int some = min(p.chunks - p.chunk, to - done);   // of this pair
+        const int lo = max(from - done, 0);
+        if (lo < some && p.grp == 0) {
+            const int g = p.g, j0 = (p.chunk + lo) * CHUNK, j1 = min((p.chunk + some) * CHUNK, p.n);
+            float* mass = c.mass + p.b * c.mass_bs + g * c.mass_hs;
+            for (int grp = 0; grp < a.groups; ++grp) {
+                const int heads = min(HG, rep - grp * HG);
+                const int64_t begin = flat - p.chunk + (int64_t)grp * (p.chunks + PT_PAD);
+                const int y0 = (int)(begin / per), y1 = (int)((begin + p.chunks - 1) / per);
+                __syncthreads();
+                for (int h = warp; h < heads; h += PJ_WARPS) { // final maximum and 1 / sum
+                    float m = -INFINITY, l = 0.f;
+                    if (y0 == y1) {
+                        const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)p.b * a.H + g * rep + grp * HG + h) * 2));
+                        m = st.x;
+                        l = st.y;
+                    } else {
+                        for (int x = y0 + lane; x <= y1; x += 32) {
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pt_part<S>(a, x, begin > x * per) + HG * DP + h * 2));
+                            const float mn = fmaxf(m, ml.x);
+                            l = l * pt_factor(m, mn) + ml.y * pt_factor(ml.x, mn);
+                            m = mn;
+                        }
 #pragma unroll
-    for (int i = 0; i < PJ_KEYS / (PJ_WARPS * 32); ++i) w[i] = 0.f;
-    for (int grp = 0; grp < a.groups; ++grp) {
-        const int heads = min(HG, rep - grp * HG);
-        PtSpan u = s;
-        u.first += (int64_t)grp * s.chunks;
-        u.last += (int64_t)grp * s.chunks;
-        const int64_t x0 = u.first / u.per, x1 = u.last / u.per;
-        for (int h = warp; h < heads; h += PJ_WARPS) {         // final maximum and 1 / sum
-            float m = -INFINITY, l = 0.f;
-            if (x0 == x1) {
-                const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)b * a.H + g * rep + grp * HG + h) * 2));
-                m = st.x;
-                l = st.y;
-            } else {
-                for (int64_t x = x0 + lane; x <= x1; x += 32) {
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(pt_part<S>(a, u, x) + HG * DP + h * 2));
-                    const float mn = fmaxf(m, ml.x);
-                    l = l * pt_factor(m, mn) + ml.y * pt_factor(ml.x, mn);
-                    m = mn;
+                        for (int o = 16; o >= 1; o >>= 1) {
+                            const float m2 = __shfl_xor_sync(FULL, m, o), l2 = __shfl_xor_sync(FULL, l, o), mn = fmaxf(m, m2);
+                            l = l * pt_factor(m, mn) + l2 * pt_factor(m2, mn);
+                            m = mn;
+                        }
+                        l = pt_inverse(l);
+                    }
+                    if (lane == 0) {
+                        stat[0][h] = m == -INFINITY ? 0.f : m;
+                        stat[1][h] = l;
+                    }
                 }
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) {
-                    const float m2 = __shfl_xor_sync(FULL, m, o), l2 = __shfl_xor_sync(FULL, l, o), mn = fmaxf(m, m2);
-                    l = l * pt_factor(m, mn) + l2 * pt_factor(m2, mn);
-                    m = mn;
+                __syncthreads();
+                const float* sc = a.scores + begin * CHUNK * a.rs;
+                if (a.rs == 4) {
+                    const float4 m4 = make_float4(stat[0][0], stat[0][1], stat[0][2], stat[0][3]);
+                    const float4 l4 = make_float4(stat[1][0], stat[1][1], stat[1][2], heads > 3 ? stat[1][3] : 0.f);
+#pragma unroll 4
+                    for (int j = j0 + t; j < j1; j += PJ_WARPS * 32) {
+                        const float4 x = __ldcs(reinterpret_cast<const float4*>(sc) + j);
+                        float w = exp2_fast(x.x - m4.x) * l4.x;
+                        w = fmaf(exp2_fast(x.y - m4.y), l4.y, w);
+                        w = fmaf(exp2_fast(x.z - m4.z), l4.z, w);
+                        if (heads > 3) w = fmaf(exp2_fast(x.w - m4.w), l4.w, w);
+                        mass[j] += w;
+                    }
+                } else {
+#pragma unroll 2
+                    for (int j = j0 + t; j < j1; j += PJ_WARPS * 32) {
+                        float w = 0.f;
+                        for (int h = 0; h < heads; ++h) w = fmaf(exp2_fast(__ldcg(sc + (int64_t)j * a.rs + h) - stat[0][h]), stat[1][h], w);
+                        mass[j] += w;
+                    }
                 }
-                l = pt_inverse(l);
-            }
-            if (lane == 0) {
-                stat[0][h] = m == -INFINITY ? 0.f : m;
-                stat[1][h] = l;
             }
         }
-        __syncthreads();
-        const float* sc = a.scores + u.first * S::CHUNK * a.rs;
-#pragma unroll
-        for (int i = 0; i < PJ_KEYS / (PJ_WARPS * 32); ++i) {
-            const int j = j0 + i * PJ_WARPS * 32 + t;
-            if (j < n)
-                for (int h = 0; h < heads; ++h) w[i] = fmaf(exp2_fast(__ldcg(sc + (int64_t)j * a.rs + h) - stat[0][h]), stat[1][h], w[i]);
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < PJ_KEYS / (PJ_WARPS * 32); ++i) {
-        const int j = j0 + i * PJ_WARPS * 32 + t;
-        if (j < n) c.mass[b * c.mass_bs + g * c.mass_hs + j] += w[i];
+        int skip = to - done - some + 1;                       // what is left from the pair's last chunk on
+        const int before = skip;
+        p.chunk += some - 1;
+        pt_step<CHUNK>(c, a, p, skip);
+        done += some - 1 + before - skip;
+        flat += some - 1 + before - skip;
     }
 }
 
 struct PtPlan {
     int groups, rs, chunk, blocks;
     bool join;
-    size_t stats, scores, total;                               // bytes in front of them, and of all
+    size_t parts, stats, scores, total;                        // bytes in front of them, and of all
 };
 template <typename S> PtPlan pt_plan(const sk_paged_cache& c, int H) {
     PtPlan p;
     const int rep = H / c.G;
     p.groups = (rep + S::HG - 1) / S::HG;
     p.rs = rep < S::HG ? (rep + 1) / 2 * 2 : S::HG;
-    const int64_t cap = (int64_t)c.width * c.page, chunks = (cap + S::CHUNK - 1) / S::CHUNK * c.B * c.G * p.groups;
+    const int64_t cap = (int64_t)c.width * c.page, chunks = ((cap + S::CHUNK - 1) / S::CHUNK + PT_PAD) * c.B * c.G * p.groups;
     const int64_t most = (int64_t)sm_count() * S::PER_SM;
     p.blocks = (int)(chunks < most ? (chunks < 1 ? 1 : chunks) : most);
     p.join = cap > S::CHUNK || c.mass != nullptr;
-    p.stats = cap > S::CHUNK ? up256((size_t)p.blocks * 2 * S::HG * (S::DP + 2) * 4) : 0;
+    p.parts = p.join ? up256((size_t)p.blocks * sizeof(PtRun)) : 0;
+    p.stats = p.parts + (cap > S::CHUNK ? up256((size_t)p.blocks * 2 * S::HG * (S::DP + 2) * 4) : 0);
     p.scores = p.stats + (c.mass != nullptr ? up256((size_t)c.B * H * 8) : 0);
     p.total = p.scores + (c.mass != nullptr ? up256((size_t)chunks * S::CHUNK * p.rs * 4) : 0);
     return p;
@@ -653,13 +739,11 @@ int launch_paged_attn(const sk_paged_cache& c, const void* q, int64_t q_bs, int6
         using S = decltype(shape);
         using T = decltype(t);
         const PtPlan p = pt_plan<S>(c, H);
-        const int64_t pieces = ((int64_t)c.width * c.page + PJ_KEYS - 1) / PJ_KEYS;
-        const int64_t joins = (int64_t)c.B * H + (c.mass != nullptr ? pieces * c.B * c.G : 0);
-        if (joins > INT32_MAX) return fail(SK_ERR_UNSUPPORTED, "sk_paged_attn: %d sequences of up to %lld keys", c.B, (long long)c.width * c.page);
         PtArgs a;
         a.q = q;
         a.out = out;
-        a.parts = (float*)workspace;
+        a.runs = p.join ? (PtRun*)workspace : nullptr;
+        a.parts = (float*)((char*)workspace + p.parts);
         a.stats = c.mass != nullptr ? (float*)((char*)workspace + p.stats) : nullptr;
         a.scores = c.mass != nullptr ? (float*)((char*)workspace + p.scores) : nullptr;
         a.q_bs = q_bs;
@@ -675,7 +759,8 @@ int launch_paged_attn(const sk_paged_cache& c, const void* q, int64_t q_bs, int6
         if (e == cudaSuccess) e = launch_after(paged_attn_kernel<S, T>, dim3(p.blocks), dim3(S::THREADS), S::SMEM, st, c, a);
         if (int rc = check_chained(e, "paged_attn_kernel")) return rc;
         if (!p.join) return SK_OK;
-        return check_chained(launch_after(paged_join_kernel<S, T>, dim3((unsigned)joins), dim3(PJ_WARPS * 32), 0, st, c, a, p.blocks), "paged_join_kernel");
+        const dim3 grid(p.blocks, S::HG + (c.mass != nullptr ? PJ_SHARES : 0));
+        return check_chained(launch_after(paged_join_kernel<S, T>, grid, dim3(PJ_WARPS * 32), 0, st, c, a), "paged_join_kernel");
     });
 }
 
