@@ -116,11 +116,11 @@ SIGNATURES = {
     "sk_rms_norm": (_i, [_p, _p, _i, _i64, _i, _f, _p, _p]),
     "sk_pick_token": (_i, [_p, _i, _i64, _i, _i, _p, _p, _p, _p]),
     "sk_begin_token": (_i, [_p, _p, _i, _p, _p, _i64, _p, _i, _p]),
-    "sk_paged_append": (_i, [C.POINTER(PagedCacheParams), _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _p, _p, _p]),
-    "sk_paged_attn_workspace_bytes": (_sz, [C.POINTER(PagedCacheParams), _i]),
-    "sk_paged_attn": (_i, [C.POINTER(PagedCacheParams), _p, _i64, _i64, _p, _i64, _i64, _i, _i, _f, _p, _sz, _p]),
-    "sk_paged_evict_workspace_bytes": (_sz, [C.POINTER(PagedCacheParams), _i]),
-    "sk_paged_evict": (_i, [C.POINTER(PagedCacheParams), _i, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _sz, _p]),
+    "sk_paged_append": (_i, [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _p, _p, _p]),
+    "sk_paged_attn_workspace_bytes": (_sz, [_p, _i]),
+    "sk_paged_attn": (_i, [_p, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _f, _p, _sz, _p]),
+    "sk_paged_evict_workspace_bytes": (_sz, [_p, _i]),
+    "sk_paged_evict": (_i, [_p, _i, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _sz, _p]),
     "sk_token_logprobs": (_i, [_p, _i, _i64, _i64, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
 }
 
@@ -276,13 +276,15 @@ def stream_ptr(device=None) -> int:
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
-def on_device(device: torch.device, check_status, entry, what: str, *args) -> None:
-    """entry(*args, stream) on the current stream of `device`, whichever device is the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        check_status(entry(*args, stream_ptr(device)), what)
-        return
-    with torch.cuda.device(device):
-        check_status(entry(*args, stream_ptr(device)), what)
+def on_device(index: int, check_status, entry, what: str, *args) -> None:
+    """entry(*args, stream) on the current stream of device `index`, whichever device is the current one."""
+    if index == torch.cuda.current_device():
+        status = entry(*args, torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, torch.cuda.current_stream(index).cuda_stream)
+    if status != 0:
+        check_status(status, what)
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -4,39 +4,50 @@
 namespace sk {
 namespace {
 
-// One warp per new row (sequence, token, head): the key's and the value's 16-byte pieces, and the slot's bookkeeping.  Nothing but
-// copies: bound by memory.
-constexpr int PA_WARPS = 8;
-__global__ void __launch_bounds__(PA_WARPS * 32)
+// A thread per 16-byte piece of four new rows (sequence, token, head) of its own: the pieces of both tensors are asked for before the
+// table is, and written behind it.  Nothing but copies: bound by memory.
+constexpr int PA_THREADS = 256, PA_ROWS = 4;
+__global__ void __launch_bounds__(PA_THREADS)
 paged_append_kernel(const __grid_constant__ sk_paged_cache c, const char* k_new, int64_t kn_bs, int64_t kn_ss, int64_t kn_hs, const char* v_new,
-                    int64_t vn_bs, int64_t vn_ss, int64_t vn_hs, int S, const int32_t* counts, const int32_t* first, int es) {
-    const int64_t row = (int64_t)blockIdx.x * PA_WARPS + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= (int64_t)c.B * S * c.G) return;
-    const int g = (int)(row % c.G), s = (int)(row / c.G % S), b = (int)(row / c.G / S);
-    if (counts != nullptr && s >= counts[b]) return;
-    const int64_t slot = (int64_t)max(c.lengths[b], 0) + s;
-    const int shift = 31 - __clz(c.page);
-    int flag = 0;
-    if (slot >= (int64_t)c.width * c.page) flag = SK_DEV_POS_OUT_OF_RANGE;
-    const int page = flag == 0 ? c.table[b * c.table_ld + (slot >> shift)] : 0;
-    if (flag == 0 && !paged_page_ok(c, page)) flag = SK_DEV_INDEX_OUT_OF_RANGE;
-    if (flag != 0) {
-        if (lane == 0 && c.status != nullptr) atomicOr(c.status, flag);
-        return;
+                    int64_t vn_bs, int64_t vn_ss, int64_t vn_hs, int S, const int32_t* counts, const int32_t* first, int es, int pieces, int rows) {
+    pdl_begin();
+    // pieces of a row, rounded up to a power of two: lanes of a row and rows of a block
+    const int per = 1 << (32 - __clz(pieces - 1)), p = threadIdx.x & (per - 1), step = PA_THREADS / per, shift = 31 - __clz(c.page);
+    const int b = blockIdx.y, r0 = blockIdx.x * PA_ROWS * step + threadIdx.x / per, n = counts != nullptr ? min(counts[b], S) : S;
+    const int64_t length = max(c.lengths[b], 0);
+    uint4 k[PA_ROWS], v[PA_ROWS];
+    int page[PA_ROWS];
+#pragma unroll
+    for (int i = 0; i < PA_ROWS; ++i) {
+        const int r = r0 + i * step, s = r / c.G, g = r - s * c.G;
+        page[i] = -1;
+        if (r >= rows || s >= n) continue;
+        const bool in = length + s < (int64_t)c.width * c.page;
+        if (in) page[i] = __ldcg(c.table + b * c.table_ld + ((length + s) >> shift));
+        else if (p == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
+        if (p < pieces) {
+            k[i] = __ldcs(reinterpret_cast<const uint4*>(k_new + (b * kn_bs + s * kn_ss + g * kn_hs) * es) + p);
+            v[i] = __ldcs(reinterpret_cast<const uint4*>(v_new + (b * vn_bs + s * vn_ss + g * vn_hs) * es) + p);
+        }
     }
-    const int r = (int)(slot & (c.page - 1)), pieces = c.D * es / 16;
-    const uint4* ks = reinterpret_cast<const uint4*>(k_new + (b * kn_bs + s * kn_ss + g * kn_hs) * es);
-    const uint4* vs = reinterpret_cast<const uint4*>(v_new + (b * vn_bs + s * vn_ss + g * vn_hs) * es);
-    uint4* kd = reinterpret_cast<uint4*>((char*)c.k + (page * c.k_ps + g * c.k_hs + r * c.k_rs) * es);
-    uint4* vd = reinterpret_cast<uint4*>((char*)c.v + (page * c.v_ps + g * c.v_hs + r * c.v_rs) * es);
-    for (int i = lane; i < pieces; i += 32) {
-        kd[i] = ks[i];
-        vd[i] = vs[i];
-    }
-    if (lane == 0) {
-        if (c.mass != nullptr) c.mass[b * c.mass_bs + g * c.mass_hs + slot] = 0.f;
-        if (c.positions != nullptr) c.positions[b * c.pos_bs + g * c.pos_hs + slot] = (int32_t)(first != nullptr ? (int64_t)first[b] + s : slot);
+#pragma unroll
+    for (int i = 0; i < PA_ROWS; ++i) {
+        const int r = r0 + i * step, s = r / c.G, g = r - s * c.G;
+        if (r >= rows || s >= n || length + s >= (int64_t)c.width * c.page) continue;
+        if (!paged_page_ok(c, page[i])) {
+            if (p == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
+            continue;
+        }
+        const int64_t slot = length + s;
+        const int in = (int)(slot & (c.page - 1));
+        if (p < pieces) {
+            reinterpret_cast<uint4*>((char*)c.k + (page[i] * c.k_ps + g * c.k_hs + in * c.k_rs) * es)[p] = k[i];
+            reinterpret_cast<uint4*>((char*)c.v + (page[i] * c.v_ps + g * c.v_hs + in * c.v_rs) * es)[p] = v[i];
+        }
+        if (p == 0) {
+            if (c.mass != nullptr) c.mass[b * c.mass_bs + g * c.mass_hs + slot] = 0.f;
+            if (c.positions != nullptr) c.positions[b * c.pos_bs + g * c.pos_hs + slot] = (int32_t)(first != nullptr ? (int64_t)first[b] + s : slot);
+        }
     }
 }
 
@@ -44,11 +55,24 @@ paged_append_kernel(const __grid_constant__ sk_paged_cache c, const char* k_new,
 
 int launch_paged_append(const sk_paged_cache& c, const void* k_new, int64_t kn_bs, int64_t kn_ss, int64_t kn_hs, const void* v_new,
                         int64_t vn_bs, int64_t vn_ss, int64_t vn_hs, int S, const int32_t* counts, const int32_t* first, cudaStream_t st) {
-    const int64_t rows = (int64_t)c.B * S * c.G, blocks = (rows + PA_WARPS - 1) / PA_WARPS;
-    if (blocks > 0x7fffffff) return fail(SK_ERR_UNSUPPORTED, "sk_paged_append: %lld rows in one call", (long long)rows);
-    paged_append_kernel<<<(unsigned)blocks, PA_WARPS * 32, 0, st>>>(c, (const char*)k_new, kn_bs, kn_ss, kn_hs, (const char*)v_new, vn_bs,
-                                                                    vn_ss, vn_hs, S, counts, first, (int)esize(c.dtype));
-    return check_launch("paged_append_kernel");
+    const int es = (int)esize(c.dtype), pieces = c.D * es / 16;
+    int per = 1;
+    while (per < pieces) per *= 2;
+    const int64_t rows = (int64_t)S * c.G, of_block = PA_ROWS * (PA_THREADS / per), blocks = (rows + of_block - 1) / of_block;
+    if (rows > INT32_MAX - 65536) return fail(SK_ERR_UNSUPPORTED, "sk_paged_append: %lld rows of a sequence in one call", (long long)rows);
+    for (int b0 = 0; b0 < c.B; b0 += 65535) {                  // the grid's second dimension
+        sk_paged_cache part = c;
+        const int n = c.B - b0 < 65535 ? c.B - b0 : 65535;
+        part.table += b0 * c.table_ld;
+        part.lengths += b0;
+        if (part.mass != nullptr) part.mass += b0 * c.mass_bs;
+        if (part.positions != nullptr) part.positions += b0 * c.pos_bs;
+        const cudaError_t e = launch_after(paged_append_kernel, dim3((unsigned)blocks, n), dim3(PA_THREADS), 0, st, part, (const char*)k_new + b0 * kn_bs * es, kn_bs, kn_ss,
+                                           kn_hs, (const char*)v_new + b0 * vn_bs * es, vn_bs, vn_ss, vn_hs, S, counts != nullptr ? counts + b0 : counts,
+                                           first != nullptr ? first + b0 : first, es, pieces, (int)rows);
+        if (int rc = check_chained(e, "paged_append_kernel")) return rc;
+    }
+    return SK_OK;
 }
 
 // What every call asks of a cache

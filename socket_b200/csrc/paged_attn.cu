@@ -755,7 +755,8 @@ int launch_paged_attn(const sk_paged_cache& c, const void* q, int64_t q_bs, int6
         a.groups = p.groups;
         a.rs = p.rs;
         a.scale = scale * PT_LOG2E;
-        cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<S, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        static SmemLimit limit;
+        cudaError_t e = limit.raise((const void*)paged_attn_kernel<S, T>, S::SMEM);
         if (e == cudaSuccess) e = launch_after(paged_attn_kernel<S, T>, dim3(p.blocks), dim3(S::THREADS), S::SMEM, st, c, a);
         if (int rc = check_chained(e, "paged_attn_kernel")) return rc;
         if (!p.join) return SK_OK;

@@ -515,7 +515,8 @@ int logprobs_launch(const void* logits, int64_t ld, int64_t rows, int vocab, con
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = CL > 1 ? 2 : 1;
-    const cudaError_t e = cudaFuncSetAttribute(token_logprobs_kernel<T, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpShared));
+    static SmemLimit limit;
+    const cudaError_t e = limit.raise((const void*)token_logprobs_kernel<T, CL>, sizeof(LpShared));
     if (e != cudaSuccess) return check_chained(e, "token_logprobs_kernel");
     return check_chained(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, CL>, (const T*)logits, ld, vocab, token, top, logprob, entropy,
                                             top_logprob, top_token, status), "token_logprobs_kernel");

@@ -133,23 +133,22 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     _require_cuda(logits)
     dev = logits.device
     _require_on(dev, tokens, status)
-    assert logits.dim() == 2
     rows, vocab = logits.shape
     if not 0 <= top <= min(TOP_TOKENS, vocab):
         raise RuntimeError(f"token_logprobs: {top} alternatives of {vocab} tokens (at most {TOP_TOKENS})")
     logits = _separate_rows(logits)                               # lives until the launch
-    found = torch.empty(2 + top, rows, dtype=torch.float32, device=dev)
-    logprobs, entropy, top_logprobs = found[0], found[1], found[2:].view(rows, top)
-    top_tokens = torch.empty(rows, top, dtype=torch.int64, device=dev)
-    if tokens is None:
-        logprobs = None
-    else:
+    logprobs, f32 = None, torch.float32
+    if tokens is not None:
         assert tokens.dtype == torch.int64 and tokens.numel() == rows
         tokens = tokens.contiguous()
-    entry = lib().sk_token_logprobs if library == "step" else blocks().skb_token_logprobs
-    on_device(dev, check if library == "step" else check_blocks, entry, "token_logprobs", logits.data_ptr(), dtype_code(logits), _ld(logits), rows,
-              vocab, ptr(tokens), top, ptr(logprobs), entropy.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr(), ptr(status))
-    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)
+        logprobs = torch.empty(rows, dtype=f32, device=dev)
+    found = TokenLogprobs(logprobs, torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, top, dtype=f32, device=dev),
+                          torch.empty(rows, top, dtype=torch.int64, device=dev))
+    step = library == "step"
+    on_device(dev.index, check if step else check_blocks, lib().sk_token_logprobs if step else blocks().skb_token_logprobs, "token_logprobs",
+              logits.data_ptr(), dtype_code(logits), _ld(logits), rows, vocab, ptr(tokens), top, ptr(logprobs), found[1].data_ptr(),
+              found[2].data_ptr(), found[3].data_ptr(), ptr(status))
+    return found
 
 
 def begin_token(first: Tensor, token: Tensor, pos: Tensor, seqlens: Tensor, position: int, lengths: Sequence[Tensor], library: str) -> None:

@@ -10,29 +10,40 @@ Nothing here synchronises with the host, and nothing has a CPU path.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import check, dtype_code, lib, on_device, ptr, stream_ptr
-from .few_rows import _require_on
-from .ops import _require_cuda
+from ._lib import check, dtype_code, lib, on_device, ptr
+
+# `sk_paged_cache` as bytes: filling in a ctypes structure field by field costs a call of a few microseconds another three
+_pack = struct.Struct("7P12q6i").pack
 
 
-def _params(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass: Optional[Tensor], positions: Optional[Tensor],
-            status: Optional[Tensor]) -> _lib.PagedCacheParams:
+def _same_device(index: int, *tensors: Optional[Tensor]) -> None:
+    """Every tensor of a call lies on the device of its pools: the kernels read and write addresses."""
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"tensors of one call on device {index} and on {t.device}")
+
+
+def _cache(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass: Optional[Tensor], positions: Optional[Tensor],
+           status: Optional[Tensor]) -> bytes:
     """The parameter block of a cache, its tensors checked."""
-    _require_cuda(k_pages)
-    dev = k_pages.device
-    _require_on(dev, v_pages, table, lengths, mass, positions, status)
-    n, G, page, D = k_pages.shape
+    index = k_pages.get_device()
+    if index < 0:
+        raise RuntimeError("socket_b200 operators need CUDA tensors (there is no CPU path)")
+    _same_device(index, v_pages, table, lengths, mass, positions, status)
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    n, G, page, D = shape
     B, width = table.shape
-    assert v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype and k_pages.stride(3) == v_pages.stride(3) == 1
-    assert table.dtype == torch.int32 and (width <= 1 or table.stride(1) == 1)
-    assert lengths.dtype == torch.int32 and lengths.shape == (B,) and lengths.is_contiguous()
+    ts = table.stride()
+    assert v_pages.shape == shape and v_pages.dtype == k_pages.dtype and ks[3] == vs[3] == 1
+    assert table.dtype == lengths.dtype == torch.int32 and (width <= 1 or ts[1] == 1)
+    assert lengths.shape == (B,) and lengths.is_contiguous()
     mb = mh = pb = ph = 0
     if mass is not None:
         assert mass.dtype == torch.float32
@@ -42,15 +53,16 @@ def _params(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, ma
         pb, ph = _book(positions, B, G, width * page)
     if status is not None:
         assert status.dtype == torch.int32 and status.numel() == 1
-    return _lib.PagedCacheParams(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), ptr(mass), ptr(positions),
-                                 ptr(status), *k_pages.stride()[:3], *v_pages.stride()[:3], table.stride(0), n, mb, mh, pb, ph,
-                                 dtype_code(k_pages), B, G, D, page, width)
+    return _pack(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), ptr(mass), ptr(positions), ptr(status),
+                 ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], n, mb, mh, pb, ph, dtype_code(k_pages), B, G, D, page, width)
 
 
 def _book(t: Tensor, B: int, G: int, slots: int) -> Tuple[int, int]:
     """Strides of what is kept per sequence, head and slot."""
-    assert t.dim() == 3 and t.shape[0] == B and t.shape[1] == G and t.shape[2] >= slots and (slots <= 1 or t.stride(2) == 1)
-    return t.stride(0), t.stride(1)
+    b, g, n = t.shape
+    s = t.stride()
+    assert b == B and g == G and n >= slots and (slots <= 1 or s[2] == 1)
+    return s[0], s[1]
 
 
 def append(k_new: Tensor, v_new: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *,
@@ -59,20 +71,21 @@ def append(k_new: Tensor, v_new: Tensor, k_pages: Tensor, v_pages: Tensor, table
     """k_new, v_new [B, S, G, D] go to the slots from lengths[b] on: all S tokens, or the first counts[b] (int32) of a padded
     batch.  Their mass starts at 0; their positions are first[b] (int32; without it the slot) and up.  `lengths` stays as it is:
     the caller adds the counts once every layer has appended.  Pages written belong to one sequence each."""
-    p = _params(k_pages, v_pages, table, lengths, mass, positions, status)
-    _require_on(k_pages.device, k_new, v_new, counts, first)
-    B, S = k_new.shape[:2]
-    assert B == p.B and k_new.shape == v_new.shape == (B, S, p.G, p.D) and k_new.dtype == v_new.dtype == k_pages.dtype
-    assert p.D == 1 or k_new.stride(3) == v_new.stride(3) == 1
+    c = _cache(k_pages, v_pages, table, lengths, mass, positions, status)
+    _same_device(k_pages.get_device(), k_new, v_new, counts, first)
+    B, S, G, D = k_new.shape
+    ks, vs = k_new.stride(), v_new.stride()
+    assert v_new.shape == k_new.shape and B == table.shape[0] and G == k_pages.shape[1] and D == k_pages.shape[3]
+    assert k_new.dtype == v_new.dtype == k_pages.dtype and ks[3] == vs[3] == 1
     for t in (counts, first):
         assert t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous())
-    on_device(k_pages.device, check, lib().sk_paged_append, "sk_paged_append", C.byref(p), k_new.data_ptr(), *k_new.stride()[:3],
-              v_new.data_ptr(), *v_new.stride()[:3], S, ptr(counts), ptr(first))
+    on_device(k_pages.get_device(), check, lib().sk_paged_append, "sk_paged_append", c, k_new.data_ptr(), ks[0], ks[1], ks[2],
+              v_new.data_ptr(), vs[0], vs[1], vs[2], S, ptr(counts), ptr(first))
 
 
 def attn_workspace(H: int, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *, mass: Optional[Tensor] = None) -> int:
     """Scratch bytes of `attn` with H query heads on this cache."""
-    return int(lib().sk_paged_attn_workspace_bytes(C.byref(_params(k_pages, v_pages, table, lengths, mass, None, None)), H))
+    return int(lib().sk_paged_attn_workspace_bytes(_cache(k_pages, v_pages, table, lengths, mass, None, None), H))
 
 
 def attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *, extra: int = 0, scale: Optional[float] = None,
@@ -82,20 +95,23 @@ def attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Te
     sequence without keys gets zeros.  `scale` defaults to 1 / sqrt(D).  With `mass` every attended slot collects its weight,
     summed over the query heads of its key/value head.  A workspace that is absent or too small is allocated; calls that may
     run at the same time need one each."""
-    p = _params(k_pages, v_pages, table, lengths, mass, None, status)
-    dev = k_pages.device
-    _require_on(dev, q, out, workspace)
-    B, H, D = q.shape
-    assert B == p.B and D == p.D and H % p.G == 0 and q.dtype == k_pages.dtype and q.stride(2) == 1
+    c = _cache(k_pages, v_pages, table, lengths, mass, None, status)
+    index = k_pages.get_device()
+    _same_device(index, q, out, workspace)
+    shape, qs = q.shape, q.stride()
+    B, H, D = shape
+    assert B == table.shape[0] and D == k_pages.shape[3] and H % k_pages.shape[1] == 0 and q.dtype == k_pages.dtype and qs[2] == 1
     if out is None:
-        out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
-    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
-    need = lib().sk_paged_attn_workspace_bytes(C.byref(p), H)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    on_device(dev, check, lib().sk_paged_attn, "sk_paged_attn", C.byref(p), q.data_ptr(), *q.stride()[:2], out.data_ptr(), *out.stride()[:2],
-              H, extra, D ** -0.5 if scale is None else float(scale), ptr(workspace),
-              0 if workspace is None else workspace.numel() * workspace.element_size())
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    os = out.stride()
+    assert out.shape == shape and out.dtype == q.dtype and os[2] == 1
+    entry = lib()
+    need = entry.sk_paged_attn_workspace_bytes(c, H)
+    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if have < need:
+        workspace, have = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    on_device(index, check, entry.sk_paged_attn, "sk_paged_attn", c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], H, extra,
+              D ** -0.5 if scale is None else float(scale), ptr(workspace), have)
     return out
 
 
@@ -107,18 +123,19 @@ def evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass
     below the budget stay, the others move into the freed ones, keys and values in place.  Returns mass, positions (0 and -1
     behind the new lengths) and lengths; `out` names the tensors that get them, (mass, positions, lengths) themselves for an
     eviction in place.  Other tensors must not overlap the inputs, nor one another.  Pages of one sequence are no other's."""
-    p = _params(k_pages, v_pages, table, lengths, mass, positions, status)
-    dev = k_pages.device
-    slots = p.width * p.page
+    c = _cache(k_pages, v_pages, table, lengths, mass, positions, status)
+    index, dev = k_pages.get_device(), k_pages.device
+    B, G, slots = table.shape[0], k_pages.shape[1], table.shape[1] * k_pages.shape[2]
     if out is None:
-        out = (torch.empty(p.B, p.G, slots, dtype=torch.float32, device=dev),
-               torch.empty(p.B, p.G, slots, dtype=torch.int32, device=dev), torch.empty_like(lengths))
+        out = (torch.empty(B, G, slots, dtype=torch.float32, device=dev), torch.empty(B, G, slots, dtype=torch.int32, device=dev),
+               torch.empty(B, dtype=torch.int32, device=dev))
     m, q, n = out
-    _require_on(dev, m, q, n)
+    _same_device(index, m, q, n)
     assert m.dtype == torch.float32 and q.dtype == n.dtype == torch.int32 and n.shape == lengths.shape and n.is_contiguous()
-    strides = (*_book(m, p.B, p.G, slots), *_book(q, p.B, p.G, slots))
-    need = lib().sk_paged_evict_workspace_bytes(C.byref(p), budget)
+    (mb, mh), (pb, ph) = _book(m, B, G, slots), _book(q, B, G, slots)
+    entry = lib()
+    need = entry.sk_paged_evict_workspace_bytes(c, budget)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    on_device(dev, check, lib().sk_paged_evict, "sk_paged_evict", C.byref(p), budget, recent, sink, m.data_ptr(), *strides[:2], q.data_ptr(),
-              *strides[2:], n.data_ptr(), ptr(ws), need)
+    on_device(index, check, entry.sk_paged_evict, "sk_paged_evict", c, budget, recent, sink, m.data_ptr(), mb, mh, q.data_ptr(), pb, ph,
+              n.data_ptr(), ptr(ws), need)
     return out
