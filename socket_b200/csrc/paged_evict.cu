@@ -1,167 +1,355 @@
 // Eviction from a paged cache by collected attention weight.
+//
+// First kernel, a cluster per (sequence, key/value head): slots are ranked by a 32-bit key that grows with their mass; the key of the
+// last slot to be kept is found by four histograms of eight bits, summed over the cluster, and equal keys go by slot.  Then every slot
+// is kept or not, and the i-th freed slot below the budget and the i-th kept one behind it are written side by side.  Second kernel: a
+// list entry is a row of K, a row of V, a mass and a position to move; sources lie behind the budget and targets below it, so
+// entries may go in any order.  Only what moves is read: mass and positions once, 256 of 4352 keys of D elements.
 #include "paged.cuh"
 
 namespace sk {
 namespace {
 
-constexpr int EV_THREADS = 1024;
-struct EvMove {
-    int from;
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 8;
+constexpr int EV_SLOTS = 24576;                                // of a block, whose keys and positions find room in shared memory
+struct alignas(16) EvMove {
+    int from, to;
     float mass;
     int pos;
-    int pad;
+};
+struct EvRow {
+    int moves, length;
+};
+
+struct EvShared {
+    uint32_t hist[2][256], total[256];
+    int newest, equal, holes, movers;                          // of this block; read by the cluster
+    int digit, need;
+    int part[3][EV_WARPS];
 };
 
 // What a slot is ranked by: slots kept for sure above all, NaN above numbers
-__device__ __forceinline__ uint32_t ev_key(float mass, bool sure) {
-    return sure ? 0xFFFFFFFFu : mass != mass ? 0xFFFFFFFEu : order_key(mass);
-}
+__device__ __forceinline__ uint32_t ev_key(float mass) { return mass != mass ? 0xFFFFFFFEu : min(order_key(mass), 0xFFFFFFFEu); }
 
-// Exclusive prefix sum over the block of one flag per thread, `total` over all
-__device__ __forceinline__ int ev_scan(bool f, int* part, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned all = __ballot_sync(FULL, f);
-    __syncthreads();
-    if (lane == 0) part[warp] = __popc(all);
-    __syncthreads();
-    int before = 0, sum = 0;
-    for (int w = 0; w < EV_THREADS / 32; ++w) {
-        if (w < warp) before += part[w];
-        sum += part[w];
+// a word of another block's shared memory, at the place `local` has in this one's
+__device__ __forceinline__ uint32_t ev_remote(const void* local, int rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+template <int CL> __device__ __forceinline__ void ev_sync() {
+    if (CL == 1) __syncthreads();
+    else {
+        cluster_arrive();
+        cluster_wait();
     }
-    total = sum;
-    return before + __popc(all & ((1u << lane) - 1));
 }
 
-// One block per (sequence, key/value head).  The budget-th largest key by four digits of eight bits, then one walk over the slots in
-// order: which stay, which go, which move where.
+template <int CL>
 __global__ void __launch_bounds__(EV_THREADS)
 paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs,
-                   int32_t* pos_out, int64_t po_bs, int64_t po_hs, EvMove* moves) {
-    __shared__ uint32_t hist[256];
-    __shared__ int part[32], newest_s, need_s;
-    __shared__ uint32_t prefix_s;
-    const int g = blockIdx.x % c.G, b = blockIdx.x / c.G, t = threadIdx.x, cap = c.width * c.page, es = c.dtype == SK_F32 ? 4 : 2;
+                   int32_t* pos_out, int64_t po_bs, int64_t po_hs, EvRow* rows, EvMove* moves, int most_moves, int room) {
+    pdl_begin();
+    extern __shared__ uint32_t ev_raw[];                       // keys, then positions of this block's slots
+    __shared__ EvShared s;
+    const int rank = CL > 1 ? blockIdx.x % CL : 0, row = blockIdx.x / CL, g = row % c.G, b = row / c.G, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int cap = c.width * c.page;
     const float* mass = c.mass + b * c.mass_bs + g * c.mass_hs;
     const int32_t* pos = c.positions + b * c.pos_bs + g * c.pos_hs;
     float* mo = mass_out + b * mo_bs + g * mo_hs;
     int32_t* po = pos_out + b * po_bs + g * po_hs;
     bool over;
     const int n = paged_length(c, b, 0, &over), kept = min(n, budget);
-    if (over && t == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
-    if (n <= budget) {
-        for (int j = t; j < cap; j += EV_THREADS) {
-            mo[j] = j < n ? mass[j] : 0.f;
-            po[j] = j < n ? pos[j] : -1;
-        }
-        return;
+    if (rank == 0 && t == 0) {
+        if (over && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
+        if (n <= budget) rows[row] = EvRow{0, kept};
     }
-    if (t == 0) newest_s = INT32_MIN;
-    __syncthreads();
-    int newest = INT32_MIN;
-    for (int j = t; j < n; j += EV_THREADS) newest = max(newest, pos[j]);
-    atomicMax(&newest_s, newest);
-    __syncthreads();
-    const int64_t late = (int64_t)newest_s - recent;
-    auto key = [&](int j) { return ev_key(mass[j], pos[j] < sink || pos[j] > late); };
-    uint32_t prefix = 0;
-    int need = budget;                                         // of the keys that share the prefix
-    for (int digit = 24; digit >= 0; digit -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (int j = t; j < n; j += EV_THREADS) {
-            const uint32_t k = key(j);
-            if (digit == 24 || k >> (digit + 8) == prefix) atomicAdd(&hist[k >> digit & 255], 1u);
-        }
-        __syncthreads();
-        if (t == 0) {
-            int left = need, d = 255;
-            while ((int)hist[d] < left) left -= hist[d--];
-            need_s = left;
-            prefix_s = prefix << 8 | d;
-        }
-        __syncthreads();
-        need = need_s;
-        prefix = prefix_s;
-        __syncthreads();
-    }
-    // every key above the prefix and the first `need` that equal it are kept
-    EvMove* mv = moves + (int64_t)blockIdx.x * budget;
-    auto walk = [&](auto&& at) {                               // at(slot, live, kept, its place among the kept equal ones known)
-        int equal = 0;
-        for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
-            const int j = j0 + t;
-            const uint32_t k = j < n ? key(j) : 0;
-            int sum;
-            const int place = ev_scan(j < n && k == prefix, part, sum);
-            at(j, j < n, j < n && (k > prefix || (k == prefix && equal + place < need)));
-            equal += sum;
-        }
-    };
-    int moved = 0;
-    walk([&](int j, bool live, bool keep) {
-        int sum;
-        const bool mover = live && keep && j >= budget;
-        const int i = ev_scan(mover, part, sum);
-        if (mover) mv[moved + i] = EvMove{j, mass[j], pos[j], 0};
-        moved += sum;
-    });
-    __syncthreads();
-    const int shift = 31 - __clz(c.page), pieces = c.D * es / 16;
-    int freed = 0;
-    walk([&](int j, bool live, bool keep) {
-        int sum;
-        const bool hole = live && !keep && j < budget;
-        const int i = freed + ev_scan(hole, part, sum);
-        freed += sum;
-        const float m = live ? mass[j] : 0.f;
-        const int p = live ? pos[j] : 0;
-        __syncthreads();
-        if (hole) {
-            const EvMove e = mv[i];
-            mo[j] = e.mass;
-            po[j] = e.pos;
-            const int from = c.table[b * c.table_ld + (e.from >> shift)], to = c.table[b * c.table_ld + (j >> shift)];
-            if (paged_page_ok(c, from) && paged_page_ok(c, to)) {
-                const int rf = e.from & (c.page - 1), rt = j & (c.page - 1);
-                const uint4* ks = (const uint4*)((const char*)c.k + (from * c.k_ps + g * c.k_hs + rf * c.k_rs) * es);
-                const uint4* vs = (const uint4*)((const char*)c.v + (from * c.v_ps + g * c.v_hs + rf * c.v_rs) * es);
-                uint4* kd = (uint4*)((char*)c.k + (to * c.k_ps + g * c.k_hs + rt * c.k_rs) * es);
-                uint4* vd = (uint4*)((char*)c.v + (to * c.v_ps + g * c.v_hs + rt * c.v_rs) * es);
-                for (int x = 0; x < pieces; ++x) {
-                    kd[x] = ks[x];
-                    vd[x] = vs[x];
-                }
-            } else if (c.status != nullptr) {
-                atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
-            }
-        } else if (live && j < budget) {
-            mo[j] = m;
-            po[j] = p;
-        }
-    });
-    __syncthreads();
-    for (int j = kept + t; j < cap; j += EV_THREADS) {
+    for (int j = n + rank * EV_THREADS + t; j < cap; j += CL * EV_THREADS) {
         mo[j] = 0.f;
         po[j] = -1;
     }
+    if (n <= budget) {                                         // the whole cluster: nothing goes
+        for (int j = rank * EV_THREADS + t; j < n; j += CL * EV_THREADS) {
+            const float m = mass[j];
+            const int p = pos[j];
+            mo[j] = m;
+            po[j] = p;
+        }
+        return;
+    }
+    const int share = (n + CL - 1) / CL, j0 = min(rank * share, n), j1 = min(j0 + share, n), count = j1 - j0;
+    const bool held = share <= room;                           // keys and positions stay on chip; else they are read again
+    uint32_t* keys = ev_raw;
+    int32_t* places = reinterpret_cast<int32_t*>(ev_raw + room);
+    if (t == 0) s.newest = INT32_MIN;
+    for (int i = t; i < 256; i += EV_THREADS) s.hist[0][i] = 0;
+    __syncthreads();
+    int newest = INT32_MIN;
+#pragma unroll 4
+    for (int i = t; i < count; i += EV_THREADS) {
+        const int p = pos[j0 + i];
+        newest = max(newest, p);
+        if (held) {
+            keys[i] = ev_key(mass[j0 + i]);
+            places[i] = p;
+        }
+    }
+    newest = __reduce_max_sync(FULL, newest);
+    if (lane == 0) atomicMax(&s.newest, newest);
+    ev_sync<CL>();
+    newest = INT32_MIN;
+    for (int k = 0; k < CL; ++k) newest = max(newest, CL == 1 ? s.newest : (int)ev_remote(&s.newest, k));
+    const int64_t late = (int64_t)newest - recent;
+    auto key = [&](int i) {                                    // of slot j0 + i
+        const int p = held ? places[i] : pos[j0 + i];
+        return p < sink || p > late ? 0xFFFFFFFFu : held ? keys[i] : ev_key(mass[j0 + i]);
+    };
+
+    // ---- the smallest key that is kept, and how many of that key
+    uint32_t prefix = 0;
+    int need = budget;
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        uint32_t* hist = s.hist[pass & 1];
+        for (int i0 = 0; i0 < count; i0 += EV_THREADS) {
+            const int i = i0 + t;
+            uint32_t k = 0;
+            if (i < count) {
+                k = key(i);
+                if (held && pass == 0) keys[i] = k;            // from now on with what is kept for sure
+            }
+            warp_hist_add(hist, k >> shift & 255, i < count && (pass == 0 || k >> shift >> 8 == prefix));
+        }
+        ev_sync<CL>();
+        if (t < 256) {
+            uint32_t sum = 0;
+            for (int x = 0; x < CL; ++x) sum += CL == 1 ? hist[t] : ev_remote(hist + t, x);
+            s.total[t] = sum;
+            s.hist[(pass + 1) & 1][t] = 0;                     // read by the others before the barrier
+        }
+        __syncthreads();
+        if (warp == 0) {                                       // lane: eight bins, the largest first
+            int mine = 0;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) mine += s.total[255 - lane * 8 - x];
+            int sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(FULL, sum, o);
+                if (lane >= o) sum += x;
+            }
+            int above = sum - mine;
+            if (above < need && sum >= need) {
+                int d = 255 - lane * 8;
+                while (above + (int)s.total[d] < need) above += s.total[d--];
+                s.digit = d;
+                s.need = need - above;
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | s.digit;
+        need = s.need;
+    }
+
+    // ---- in slot order, a run of slots per warp: kept equal keys, freed slots, kept slots behind the budget
+    const int run = (count + EV_WARPS * 32 - 1) / (EV_WARPS * 32) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
+    auto before = [&](int which, int mine, int& all) {         // sum over the warps in front; `all`: over the block
+        __syncthreads();
+        if (lane == 0) s.part[which][warp] = mine;
+        __syncthreads();
+        const int x = lane < EV_WARPS ? s.part[which][lane] : 0;
+        all = __reduce_add_sync(FULL, x);
+        return __reduce_add_sync(FULL, lane < warp ? x : 0);
+    };
+    int equal = 0, all;
+    for (int i = i0 + lane; i - lane < i1; i += 32) equal += __popc(__ballot_sync(FULL, i < i1 && key(i) == prefix));
+    int equal_at = before(0, equal, all);
+    if (CL > 1) {
+        if (t == 0) s.equal = all;
+        ev_sync<CL>();
+        for (int x = 0; x < rank; ++x) equal_at += (int)ev_remote(&s.equal, x);
+    }
+    // one step of the walk over a warp's run: is slot i kept
+    auto keeps = [&](int i, int& seen) {
+        const uint32_t k = i < i1 ? key(i) : 0u;
+        const unsigned same = __ballot_sync(FULL, i < i1 && k == prefix);
+        const bool keep = i < i1 && (k > prefix || (k == prefix && seen + __popc(same & ((1u << lane) - 1)) < need));
+        seen += __popc(same);
+        return keep;
+    };
+    int holes = 0, movers = 0, seen = equal_at;
+    for (int i = i0 + lane; i - lane < i1; i += 32) {
+        const bool keep = keeps(i, seen), low = j0 + i < budget;
+        holes += __popc(__ballot_sync(FULL, i < i1 && !keep && low));
+        movers += __popc(__ballot_sync(FULL, keep && !low));
+    }
+    int all_holes, all_movers, hole_at = before(1, holes, all_holes), mover_at = before(2, movers, all_movers);
+    if (CL > 1) {
+        if (t == 0) {
+            s.holes = all_holes;
+            s.movers = all_movers;
+        }
+        ev_sync<CL>();
+        int sum = 0;
+        for (int x = 0; x < CL; ++x) {
+            const int h = (int)ev_remote(&s.holes, x), m = (int)ev_remote(&s.movers, x);
+            if (x < rank) {
+                hole_at += h;
+                mover_at += m;
+            }
+            sum += m;
+        }
+        all_movers = sum;
+    }
+    if (rank == 0 && t == 0) rows[row] = EvRow{all_movers, kept};
+    EvMove* list = moves + (int64_t)row * most_moves;
+    seen = equal_at;
+    for (int i = i0 + lane; i - lane < i1; i += 32) {
+        const bool keep = keeps(i, seen), low = j0 + i < budget, hole = i < i1 && !keep && low, mover = keep && !low;
+        const unsigned h = __ballot_sync(FULL, hole), v = __ballot_sync(FULL, mover);
+        const int j = j0 + i;
+        if (hole) list[hole_at + __popc(h & ((1u << lane) - 1))].to = j;
+        if (keep) {
+            const float m = mass[j];
+            const int p = held ? places[i] : pos[j];
+            if (mover) {
+                EvMove* e = list + mover_at + __popc(v & ((1u << lane) - 1));
+                e->from = j;
+                e->mass = m;
+                e->pos = p;
+            } else {
+                mo[j] = m;
+                po[j] = p;
+            }
+        }
+        if (i < i1 && !low) {
+            mo[j] = 0.f;
+            po[j] = -1;
+        }
+        hole_at += __popc(h);
+        mover_at += __popc(v);
+    }
+    if (CL > 1) ev_sync<CL>();                                 // no block leaves while others read its counts
 }
 
-__global__ void paged_evict_lengths_kernel(const __grid_constant__ sk_paged_cache c, int budget, int32_t* lengths_out) {
-    const int b = blockIdx.x * blockDim.x + threadIdx.x;
-    if (b < c.B) lengths_out[b] = min(paged_length(c, b, 0), budget);
+// A thread per 16-byte piece of four moves of its own
+constexpr int EM_THREADS = 256, EM_MOVES = 4;
+__global__ void __launch_bounds__(EM_THREADS)
+paged_move_kernel(const __grid_constant__ sk_paged_cache c, float* mass_out, int64_t mo_bs, int64_t mo_hs, int32_t* pos_out, int64_t po_bs, int64_t po_hs,
+                  int32_t* lengths_out, const EvRow* rows, const EvMove* moves, int most_moves, int es, int pieces, int blocks) {
+    pdl_begin();
+    const int row = blockIdx.x / blocks, part = blockIdx.x % blocks, g = row % c.G, b = row / c.G;
+    const int n = __ldcg(&rows[row].moves);
+    if (part == 0 && g == 0 && threadIdx.x == 0) lengths_out[b] = __ldcg(&rows[row].length);
+    const int per = 1 << (32 - __clz(pieces - 1)), p = threadIdx.x & (per - 1), step = EM_THREADS / per, shift = 31 - __clz(c.page);
+    const int i0 = part * EM_MOVES * step + threadIdx.x / per;
+    if (part * EM_MOVES * step >= n) return;
+    const EvMove* list = moves + (int64_t)row * most_moves;
+    int4 e[EM_MOVES];
+    int from[EM_MOVES], to[EM_MOVES];
+#pragma unroll
+    for (int x = 0; x < EM_MOVES; ++x)
+        if (i0 + x * step < n) e[x] = __ldcg(reinterpret_cast<const int4*>(list + i0 + x * step));
+#pragma unroll
+    for (int x = 0; x < EM_MOVES; ++x)
+        if (i0 + x * step < n) {
+            from[x] = __ldcg(c.table + b * c.table_ld + (e[x].x >> shift));
+            to[x] = __ldcg(c.table + b * c.table_ld + (e[x].y >> shift));
+        }
+    uint4 k[EM_MOVES], v[EM_MOVES];
+    bool ok[EM_MOVES];
+#pragma unroll
+    for (int x = 0; x < EM_MOVES; ++x) {
+        ok[x] = i0 + x * step < n && paged_page_ok(c, from[x]) && paged_page_ok(c, to[x]);
+        if (ok[x] && p < pieces) {
+            const int r = e[x].x & (c.page - 1);
+            k[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.k + (from[x] * c.k_ps + g * c.k_hs + r * c.k_rs) * es) + p);
+            v[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.v + (from[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es) + p);
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < EM_MOVES; ++x) {
+        if (i0 + x * step >= n) continue;
+        if (ok[x] && p < pieces) {
+            const int r = e[x].y & (c.page - 1);
+            reinterpret_cast<uint4*>((char*)c.k + (to[x] * c.k_ps + g * c.k_hs + r * c.k_rs) * es)[p] = k[x];
+            reinterpret_cast<uint4*>((char*)c.v + (to[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es)[p] = v[x];
+        }
+        if (p == 0) {
+            mass_out[b * mo_bs + g * mo_hs + e[x].y] = __int_as_float(e[x].z);
+            pos_out[b * po_bs + g * po_hs + e[x].y] = e[x].w;
+            if (!ok[x] && c.status != nullptr) atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
+        }
+    }
+}
+
+struct EvPlan {
+    int cluster, room, most_moves;
+    size_t moves, total;                                       // bytes in front of the lists, and of all
+};
+EvPlan ev_plan(const sk_paged_cache& c, int budget) {
+    EvPlan p;
+    const int64_t rows = (int64_t)c.B * c.G, cap = (int64_t)c.width * c.page;
+    // blocks of a row: while they find a place at once, two an SM, and have four slots a thread; more where its slots have no room on chip
+    p.cluster = 1;
+    while (p.cluster < EV_CLUSTER && ((rows * 2 * p.cluster <= 2 * sm_count() && cap >= (int64_t)8 * EV_THREADS * p.cluster) ||
+                                      (cap + p.cluster - 1) / p.cluster > EV_SLOTS))
+        p.cluster *= 2;
+    const int64_t share = (cap + p.cluster - 1) / p.cluster;
+    p.room = (int)(share < EV_SLOTS ? share : EV_SLOTS);
+    const int64_t behind = cap > budget ? cap - budget : 0;
+    p.most_moves = (int)(behind < budget ? behind : budget);
+    p.moves = up256((size_t)rows * sizeof(EvRow));
+    p.total = p.moves + (size_t)rows * p.most_moves * sizeof(EvMove);
+    return p;
+}
+
+template <int CL>
+int evict_launch(const sk_paged_cache& c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs, int32_t* pos_out,
+                 int64_t po_bs, int64_t po_hs, EvRow* rows, EvMove* moves, const EvPlan& p, cudaStream_t st) {
+    static SmemLimit limit;
+    cudaError_t e = limit.raise((const void*)paged_evict_kernel<CL>, (size_t)EV_SLOTS * 8);
+    if (e != cudaSuccess) return check_chained(e, "paged_evict_kernel");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(c.B * c.G * CL));
+    cfg.blockDim = dim3(EV_THREADS);
+    cfg.dynamicSmemBytes = (size_t)p.room * 8;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CL;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CL > 1 ? 2 : 1;
+    return check_chained(cudaLaunchKernelEx(&cfg, paged_evict_kernel<CL>, c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, rows,
+                                            moves, p.most_moves, p.room), "paged_evict_kernel");
 }
 
 }  // namespace
 
-size_t paged_evict_workspace(const sk_paged_cache& c, int budget) { return (size_t)c.B * c.G * budget * sizeof(EvMove); }
+size_t paged_evict_workspace(const sk_paged_cache& c, int budget) { return ev_plan(c, budget).total; }
 
 int launch_paged_evict(const sk_paged_cache& c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs,
                        int32_t* pos_out, int64_t po_bs, int64_t po_hs, int32_t* lengths_out, void* workspace, cudaStream_t st) {
-    paged_evict_kernel<<<c.B * c.G, EV_THREADS, 0, st>>>(c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, (EvMove*)workspace);
-    if (int rc = check_launch("paged_evict_kernel")) return rc;
-    paged_evict_lengths_kernel<<<(c.B + 255) / 256, 256, 0, st>>>(c, budget, lengths_out);
-    return check_launch("paged_evict_lengths_kernel");
+    const EvPlan p = ev_plan(c, budget);
+    EvRow* rows = (EvRow*)workspace;
+    EvMove* moves = (EvMove*)((char*)workspace + p.moves);
+    const int es = (int)esize(c.dtype), pieces = c.D * es / 16;
+    int per = 1;
+    while (per < pieces) per *= 2;
+    const int of_block = EM_MOVES * (EM_THREADS / per);
+    const int blocks = p.most_moves > 0 ? (p.most_moves + of_block - 1) / of_block : 1;
+    if ((int64_t)c.B * c.G * blocks > INT32_MAX || (int64_t)c.B * c.G * EV_CLUSTER > INT32_MAX)
+        return fail(SK_ERR_UNSUPPORTED, "sk_paged_evict: %d sequences with %d heads and a budget of %d", c.B, c.G, budget);
+    auto go = p.cluster == 8 ? evict_launch<8> : p.cluster == 4 ? evict_launch<4> : p.cluster == 2 ? evict_launch<2> : evict_launch<1>;
+    if (int rc = go(c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, rows, moves, p, st)) return rc;
+    return check_chained(launch_after(paged_move_kernel, dim3((unsigned)(c.B * c.G * blocks)), dim3(EM_THREADS), 0, st, c, mass_out, mo_bs, mo_hs, pos_out,
+                                      po_bs, po_hs, lengths_out, (const EvRow*)rows, (const EvMove*)moves, p.most_moves, es, pieces, blocks),
+                         "paged_move_kernel");
 }
 
 }  // namespace sk
