@@ -7,6 +7,8 @@
 // entries may go in any order.  Only what moves is read: mass and positions once, 256 of 4352 keys of D elements.
 #include "paged.cuh"
 
+#include <type_traits>
+
 namespace sk {
 namespace {
 
@@ -23,8 +25,8 @@ struct EvRow {
 
 struct EvShared {
     uint32_t hist[2][256], total[256];
-    int newest, equal, holes, movers;                          // of this block; read by the cluster
-    int digit, need;
+    int newest, equals, holes, movers;                         // of this block; read by the cluster
+    int digit, need, equal;
     int part[3][EV_WARPS];
 };
 
@@ -79,158 +81,179 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         return;
     }
     const int share = (n + CL - 1) / CL, j0 = min(rank * share, n), j1 = min(j0 + share, n), count = j1 - j0;
-    const bool held = share <= room;                           // keys and positions stay on chip; else they are read again
-    uint32_t* keys = ev_raw;
-    int32_t* places = reinterpret_cast<int32_t*>(ev_raw + room);
     if (t == 0) s.newest = INT32_MIN;
     for (int i = t; i < 256; i += EV_THREADS) s.hist[0][i] = 0;
     __syncthreads();
-    int newest = INT32_MIN;
+    auto select = [&](auto on_chip) {
+        constexpr bool HELD = decltype(on_chip)::value;        // keys and positions in shared memory; else they are read again
+        uint32_t* keys = ev_raw;
+        int32_t* places = reinterpret_cast<int32_t*>(ev_raw + room);
+        int newest = INT32_MIN;
 #pragma unroll 4
-    for (int i = t; i < count; i += EV_THREADS) {
-        const int p = pos[j0 + i];
-        newest = max(newest, p);
-        if (held) {
-            keys[i] = ev_key(mass[j0 + i]);
-            places[i] = p;
+        for (int i = t; i < count; i += EV_THREADS) {
+            const int p = pos[j0 + i];
+            newest = max(newest, p);
+            if (HELD) {
+                keys[i] = ev_key(mass[j0 + i]);
+                places[i] = p;
+            }
         }
-    }
-    newest = __reduce_max_sync(FULL, newest);
-    if (lane == 0) atomicMax(&s.newest, newest);
-    ev_sync<CL>();
-    newest = INT32_MIN;
-    for (int k = 0; k < CL; ++k) newest = max(newest, CL == 1 ? s.newest : (int)ev_remote(&s.newest, k));
-    const int64_t late = (int64_t)newest - recent;
-    auto key = [&](int i) {                                    // of slot j0 + i
-        const int p = held ? places[i] : pos[j0 + i];
-        return p < sink || p > late ? 0xFFFFFFFFu : held ? keys[i] : ev_key(mass[j0 + i]);
-    };
+        newest = __reduce_max_sync(FULL, newest);
+        if (lane == 0) atomicMax(&s.newest, newest);
+        ev_sync<CL>();
+        newest = s.newest;
+        if (CL > 1)
+            for (int k = 0; k < CL; ++k) newest = max(newest, (int)ev_remote(&s.newest, k));
+        const int late = (int)max((int64_t)newest - recent, (int64_t)INT32_MIN);
+        auto sure = [&](int p) { return p < sink || p > late; };
+        auto key = [&](int i) {                                // of slot j0 + i, after the first pass
+            return HELD ? keys[i] : sure(pos[j0 + i]) ? 0xFFFFFFFFu : ev_key(mass[j0 + i]);
+        };
 
-    // ---- the smallest key that is kept, and how many of that key
-    uint32_t prefix = 0;
-    int need = budget;
-#pragma unroll 1
-    for (int pass = 0; pass < 4; ++pass) {
-        const int shift = 24 - 8 * pass;
-        uint32_t* hist = s.hist[pass & 1];
-        for (int i0 = 0; i0 < count; i0 += EV_THREADS) {
+        // ---- the smallest key that is kept, and how many of that key
+        uint32_t prefix = 0;
+        int need = budget;
+        for (int i0 = 0; i0 < count; i0 += EV_THREADS) {       // masses share few exponents: equal bins are added up in the warp
             const int i = i0 + t;
             uint32_t k = 0;
             if (i < count) {
-                k = key(i);
-                if (held && pass == 0) keys[i] = k;            // from now on with what is kept for sure
+                k = HELD ? (sure(places[i]) ? 0xFFFFFFFFu : keys[i]) : key(i);
+                if (HELD) keys[i] = k;
             }
-            warp_hist_add(hist, k >> shift & 255, i < count && (pass == 0 || k >> shift >> 8 == prefix));
+            warp_hist_add(s.hist[0], k >> 24, i < count);
         }
-        ev_sync<CL>();
-        if (t < 256) {
-            uint32_t sum = 0;
-            for (int x = 0; x < CL; ++x) sum += CL == 1 ? hist[t] : ev_remote(hist + t, x);
-            s.total[t] = sum;
-            s.hist[(pass + 1) & 1][t] = 0;                     // read by the others before the barrier
-        }
-        __syncthreads();
-        if (warp == 0) {                                       // lane: eight bins, the largest first
-            int mine = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 4; ++pass) {
+            uint32_t* hist = s.hist[pass & 1];
+            if (pass > 0) {
+                const int shift = 24 - 8 * pass;
+#pragma unroll 4
+                for (int i = t; i < count; i += EV_THREADS) {
+                    const uint32_t k = key(i);
+                    if (k >> shift >> 8 == prefix) atomicAdd(&hist[k >> shift & 255], 1u);
+                }
+            }
+            ev_sync<CL>();
+            if (t < 256) {
+                uint32_t sum = hist[t];
+                if (CL > 1) {
+                    sum = 0;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) mine += s.total[255 - lane * 8 - x];
-            int sum = mine;
+                    for (int x = 0; x < CL; ++x) sum += ev_remote(hist + t, x);
+                }
+                s.total[t] = sum;
+                s.hist[(pass + 1) & 1][t] = 0;                 // read by the others before the barrier
+            }
+            __syncthreads();
+            if (warp == 0) {                                   // lane: eight bins, the largest first
+                int mine = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(FULL, sum, o);
-                if (lane >= o) sum += x;
+                for (int x = 0; x < 8; ++x) mine += s.total[255 - lane * 8 - x];
+                int sum = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(FULL, sum, o);
+                    if (lane >= o) sum += x;
+                }
+                int above = sum - mine;
+                if (above < need && sum >= need) {
+                    int d = 255 - lane * 8;
+                    while (above + (int)s.total[d] < need) above += s.total[d--];
+                    s.digit = d;
+                    s.need = need - above;
+                    s.equal = s.total[d];
+                }
             }
-            int above = sum - mine;
-            if (above < need && sum >= need) {
-                int d = 255 - lane * 8;
-                while (above + (int)s.total[d] < need) above += s.total[d--];
-                s.digit = d;
-                s.need = need - above;
-            }
+            __syncthreads();
+            prefix = prefix << 8 | s.digit;
+            need = s.need;
         }
-        __syncthreads();
-        prefix = prefix << 8 | s.digit;
-        need = s.need;
-    }
+        const bool ties = s.equal > need;                      // only some of the equal keys are kept: the first ones
 
-    // ---- in slot order, a run of slots per warp: kept equal keys, freed slots, kept slots behind the budget
-    const int run = (count + EV_WARPS * 32 - 1) / (EV_WARPS * 32) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
-    auto before = [&](int which, int mine, int& all) {         // sum over the warps in front; `all`: over the block
-        __syncthreads();
-        if (lane == 0) s.part[which][warp] = mine;
-        __syncthreads();
-        const int x = lane < EV_WARPS ? s.part[which][lane] : 0;
-        all = __reduce_add_sync(FULL, x);
-        return __reduce_add_sync(FULL, lane < warp ? x : 0);
-    };
-    int equal = 0, all;
-    for (int i = i0 + lane; i - lane < i1; i += 32) equal += __popc(__ballot_sync(FULL, i < i1 && key(i) == prefix));
-    int equal_at = before(0, equal, all);
-    if (CL > 1) {
-        if (t == 0) s.equal = all;
-        ev_sync<CL>();
-        for (int x = 0; x < rank; ++x) equal_at += (int)ev_remote(&s.equal, x);
-    }
-    // one step of the walk over a warp's run: is slot i kept
-    auto keeps = [&](int i, int& seen) {
-        const uint32_t k = i < i1 ? key(i) : 0u;
-        const unsigned same = __ballot_sync(FULL, i < i1 && k == prefix);
-        const bool keep = i < i1 && (k > prefix || (k == prefix && seen + __popc(same & ((1u << lane) - 1)) < need));
-        seen += __popc(same);
-        return keep;
-    };
-    int holes = 0, movers = 0, seen = equal_at;
-    for (int i = i0 + lane; i - lane < i1; i += 32) {
-        const bool keep = keeps(i, seen), low = j0 + i < budget;
-        holes += __popc(__ballot_sync(FULL, i < i1 && !keep && low));
-        movers += __popc(__ballot_sync(FULL, keep && !low));
-    }
-    int all_holes, all_movers, hole_at = before(1, holes, all_holes), mover_at = before(2, movers, all_movers);
-    if (CL > 1) {
-        if (t == 0) {
-            s.holes = all_holes;
-            s.movers = all_movers;
-        }
-        ev_sync<CL>();
-        int sum = 0;
-        for (int x = 0; x < CL; ++x) {
-            const int h = (int)ev_remote(&s.holes, x), m = (int)ev_remote(&s.movers, x);
-            if (x < rank) {
-                hole_at += h;
-                mover_at += m;
+        // ---- in slot order, a run of slots per warp: freed slots, kept slots behind the budget
+        const int run = (count + EV_WARPS * 32 - 1) / (EV_WARPS * 32) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
+        auto before = [&](int which, int mine, int& all) {     // sum over the warps in front; `all`: over the block
+            if (lane == 0) s.part[which][warp] = mine;
+            __syncthreads();
+            const int x = lane < EV_WARPS ? s.part[which][lane] : 0;
+            all = __reduce_add_sync(FULL, x);
+            return __reduce_add_sync(FULL, lane < warp ? x : 0);
+        };
+        int equal_at = 0, all;
+        if (ties) {
+            int equal = 0;
+            for (int i = i0 + lane; i - lane < i1; i += 32) equal += __popc(__ballot_sync(FULL, i < i1 && key(i) == prefix));
+            equal_at = before(0, equal, all);
+            if (CL > 1) {
+                if (t == 0) s.equals = all;
+                ev_sync<CL>();
+                for (int x = 0; x < rank; ++x) equal_at += (int)ev_remote(&s.equals, x);
             }
-            sum += m;
         }
-        all_movers = sum;
-    }
-    if (rank == 0 && t == 0) rows[row] = EvRow{all_movers, kept};
-    EvMove* list = moves + (int64_t)row * most_moves;
-    seen = equal_at;
-    for (int i = i0 + lane; i - lane < i1; i += 32) {
-        const bool keep = keeps(i, seen), low = j0 + i < budget, hole = i < i1 && !keep && low, mover = keep && !low;
-        const unsigned h = __ballot_sync(FULL, hole), v = __ballot_sync(FULL, mover);
-        const int j = j0 + i;
-        if (hole) list[hole_at + __popc(h & ((1u << lane) - 1))].to = j;
-        if (keep) {
-            const float m = mass[j];
-            const int p = held ? places[i] : pos[j];
+        // one step of the walk over a warp's run: is slot i kept
+        auto keeps = [&](int i, int& seen) {
+            const uint32_t k = i < i1 ? key(i) : 0u;
+            if (!ties) return i < i1 && k >= prefix;
+            const unsigned same = __ballot_sync(FULL, i < i1 && k == prefix);
+            const bool keep = i < i1 && (k > prefix || (k == prefix && seen + __popc(same & ((1u << lane) - 1)) < need));
+            seen += __popc(same);
+            return keep;
+        };
+        const int low = budget - j0;                           // slots of this block below the budget
+        int holes = 0, movers = 0, seen = equal_at;
+        for (int i = i0 + lane; i - lane < i1; i += 32) {
+            const bool keep = keeps(i, seen);
+            holes += i < i1 && !keep && i < low;
+            movers += keep && i >= low;
+        }
+        holes = __reduce_add_sync(FULL, holes);
+        movers = __reduce_add_sync(FULL, movers);
+        int all_holes, all_movers, hole_at = before(1, holes, all_holes), mover_at = before(2, movers, all_movers);
+        if (CL > 1) {
+            if (t == 0) {
+                s.holes = all_holes;
+                s.movers = all_movers;
+            }
+            ev_sync<CL>();
+            int sum = 0;
+#pragma unroll
+            for (int x = 0; x < CL; ++x) {
+                const int h = (int)ev_remote(&s.holes, x), m = (int)ev_remote(&s.movers, x);
+                if (x < rank) {
+                    hole_at += h;
+                    mover_at += m;
+                }
+                sum += m;
+            }
+            all_movers = sum;
+        }
+        if (rank == 0 && t == 0) rows[row] = EvRow{all_movers, kept};
+        EvMove* list = moves + (int64_t)row * most_moves;
+        seen = equal_at;
+#pragma unroll 2
+        for (int i = i0 + lane; i - lane < i1; i += 32) {
+            const int j = j0 + i;
+            const float m = i < i1 ? mass[j] : 0.f;
+            const int p = i < i1 ? (HELD ? places[i] : pos[j]) : 0;
+            const bool keep = keeps(i, seen), hole = i < i1 && !keep && i < low, mover = keep && i >= low;
+            const unsigned h = __ballot_sync(FULL, hole), v = __ballot_sync(FULL, mover);
+            if (hole) list[hole_at + __popc(h & ((1u << lane) - 1))].to = j;
             if (mover) {
                 EvMove* e = list + mover_at + __popc(v & ((1u << lane) - 1));
                 e->from = j;
                 e->mass = m;
                 e->pos = p;
-            } else {
-                mo[j] = m;
-                po[j] = p;
             }
+            if (i < i1 && !hole) {                             // a hole's are written with the move
+                mo[j] = i < low ? m : 0.f;
+                po[j] = i < low ? p : -1;
+            }
+            hole_at += __popc(h);
+            mover_at += __popc(v);
         }
-        if (i < i1 && !low) {
-            mo[j] = 0.f;
-            po[j] = -1;
-        }
-        hole_at += __popc(h);
-        mover_at += __popc(v);
-    }
+    };
+    if (share <= room) select(std::true_type{});
+    else select(std::false_type{});
     if (CL > 1) ev_sync<CL>();                                 // no block leaves while others read its counts
 }
 
