@@ -50,6 +50,9 @@ class Decoder(nn.Module):
     def _decode_logits(self, mode: str) -> Tensor:
         raise NotImplementedError
 
+    def choose_mode(self, mode: Optional[str]) -> None:
+        """Called before the caches of a generation are made, with the mode that will decode (None: the default)."""
+
     def _setup_decode_layers(self, batch: int, mode: str) -> None:
         pass
 
@@ -109,6 +112,25 @@ class Decoder(nn.Module):
             want = None if s1 == T else ()
             logits = self.forward_portion(idx[:, s0:s1], s0, want)
         return logits[:, -1]
+
+    @torch.no_grad()
+    def score(self, idx: Tensor, top: int = 0, chunk: int = 8192) -> few_rows.TokenLogprobs:
+        """How likely a prompt's tokens are, idx [B,T]: log probability of tokens 1 .. T - 1 under what stands in front of each
+        ([B, T - 1]), the entropy of their distributions and the `top` likeliest tokens ([B, T - 1, top]).  The prompt is processed
+        and cached as by `prefill`."""
+        B, T = idx.shape
+        assert 2 <= T <= self.max_seq_length and B <= self.max_batch_size
+        parts = []
+        for s0 in range(0, T, chunk):
+            x = self._portion(idx[:, s0:min(T, s0 + chunk)], s0)
+            rows = max(1, 2048 // B)                         # logits of 2048 tokens at a time
+            for r in range(0, min(x.shape[1], T - 1 - s0), rows):
+                n = min(rows, T - 1 - s0 - r, x.shape[1] - r)
+                logits = self._head(x[:, r:r + n].contiguous())
+                given = idx[:, s0 + r + 1:s0 + r + 1 + n].reshape(-1)
+                found = few_rows.token_logprobs(logits.reshape(B * n, -1), given, top=top, library=self.libraries[0])
+                parts.append([t.view(B, n, *t.shape[1:]) for t in found])
+        return few_rows.TokenLogprobs(*(torch.cat(p, 1) for p in zip(*parts)))
 
     # -- decode ----------------------------------------------------------------------------
     def _decode_body(self, mode: str) -> None:
@@ -203,16 +225,19 @@ class Decoder(nn.Module):
 
 @torch.no_grad()
 def generate(model: Decoder, prompt: Tensor, max_new_tokens: int, mode: Optional[str] = None,
-             prefill_chunk: int = 8192, use_graph: bool = True, stream_to_host: bool = False):
+             prefill_chunk: int = 8192, use_graph: bool = True, stream_to_host: bool = False, logprobs: Optional[int] = None):
     """Greedy generation as GPT-FAST/generate.py:246-370: prefill the prompt, take the first new
     token from the prefill logits, then `max_new_tokens - 1` decode steps.  Returns (tokens
     [B, T + max_new_tokens], stats) with `decode_time_s` measured by CUDA events around the decode
     loop and `decode_only_tokens = B * (max_new_tokens - 1)` (generate.py:362-368).  `prompt` may be
     a host tensor; with `stream_to_host` every new token is copied to pinned host memory and waited
-    for before the next step is launched (the end-to-end serving pattern)."""
+    for before the next step is launched (the end-to-end serving pattern).  With `logprobs` (a number of alternatives, 0 for none)
+stats["logprobs"] tells how likely the new tokens were: log probabilities and entropies [B, max_new_tokens], and the likeliest
+tokens with theirs [B, max_new_tokens, logprobs]."""
     dev = model.device
     B, T = prompt.shape
     prompt_d = prompt.to(dev, non_blocking=True)
+    model.choose_mode(mode)
     model.setup_caches(B, T + max_new_tokens + 8)
     cuda = dev.type == "cuda"
     e = [torch.cuda.Event(enable_timing=True) for _ in range(4)] if cuda else None
@@ -228,6 +253,13 @@ def generate(model: Decoder, prompt: Tensor, max_new_tokens: int, mode: Optional
     seq[:, :T] = prompt_d
     seq[:, T] = first[:, 0]
     model.start_decode(first, T)
+    likely = []
+
+    def note(logits, tok):
+        if logprobs is not None:
+            likely.append(few_rows.token_logprobs(logits, tok, top=logprobs, library=model.libraries[0]))
+
+    note(logits, first)
     host_tok = torch.empty(B, 1, dtype=torch.long).pin_memory() if (cuda and stream_to_host) else None
     if cuda:
         torch.cuda.synchronize(dev)
@@ -235,10 +267,13 @@ def generate(model: Decoder, prompt: Tensor, max_new_tokens: int, mode: Optional
     for i in range(1, max_new_tokens):
         tok = model.decode_one_token()
         seq[:, T + i] = tok[:, 0]
+        note(model._logits, tok)
         if host_tok is not None:
             host_tok.copy_(tok, non_blocking=True)
             torch.cuda.current_stream(dev).synchronize()
     stats = {"decode_only_tokens": B * max(0, max_new_tokens - 1)}
+    if logprobs is not None:
+        stats["logprobs"] = few_rows.TokenLogprobs(*(torch.stack(t, 1) for t in zip(*likely)))
     if cuda:
         e[3].record()
         torch.cuda.synchronize(dev)

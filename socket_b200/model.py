@@ -20,7 +20,8 @@ What differs from the reference, on purpose:
 A decode step's projections and norms run on the kernels of `few_rows.py` (one GPU, at most 8 rows of a 16-bit
 type); other GEMMs and norms and the dense baseline attention are torch / library kernels: they surround the
 path, they are not it.  `mode="dense"` attends over the whole cache with a split-KV flash decode
-and is the full-attention baseline of the tokens/s comparison.
+and is the full-attention baseline of the tokens/s comparison.  `mode="paged"` (`Transformer.use_pages`) keeps the caches in
+pages and attends over them with `paged.attn`; with a budget it evicts the keys that got the least weight.
 """
 from __future__ import annotations
 
@@ -35,6 +36,7 @@ from torch import Tensor
 from . import few_rows, ops, tp
 from .attention import KVCache
 from .decoder import Decoder, find_multiple, generate  # noqa: F401  (generate: the public entry point)
+from .paged import PagedKVCache, PageTable, Paging
 from .synth import hypercube_protos
 
 
@@ -219,6 +221,7 @@ class Attention(nn.Module):
                              else torch.randn(self.K, self.R))
         self.world = world
         self.kv_cache: Optional[KVCache] = None
+        self.workspace: Optional[Tensor] = None       # scratch of attention over pages, shared by all layers
         self._step = None
 
     # ---- prefill: dense causal attention of a chunk of the prompt against the cache
@@ -229,6 +232,11 @@ class Attention(nn.Module):
         k = apply_rotary_emb(k.view(B, S, self.n_local_heads, self.head_dim), freqs_cis)
         v = v.view(B, S, self.n_local_heads, self.head_dim)
         cache = self.kv_cache
+        if isinstance(cache, PagedKVCache):
+            cache.append(k, v)
+            done = cache.pages.length                   # cached tokens, fewer than `start` after an eviction
+            keys, values = cache.rows(done + S) if done else (k.transpose(1, 2), v.transpose(1, 2))
+            return self.wo(_causal_attention(q, keys, values, done).reshape(B, S, self.local_dim))
         if x.is_cuda:
             cache.append(input_pos, k.contiguous(), v.contiguous(), self.planes.to(k.dtype))
         else:                                           # CPU: dense reference flow only (tests)
@@ -246,6 +254,9 @@ class Attention(nn.Module):
         self.v_s = torch.empty(batch, 1, self.n_local_heads, self.head_dim, dtype=dt, device=dev)
         self.o_s = torch.empty(batch, self.n_head, self.head_dim, dtype=dt, device=dev)
         self._step = None
+        paged = isinstance(self.kv_cache, PagedKVCache)
+        if paged != (mode == "paged"):
+            raise RuntimeError(f"mode {mode!r} on caches that are {'' if paged else 'not '}in pages: see Transformer.use_pages")
         if mode == "sparse":
             cache = self.kv_cache
             self._step = ops.DecodeStep(cache, self.q_s, self.k_s, self.v_s, pos, self.planes.to(dt),
@@ -272,6 +283,9 @@ class Attention(nn.Module):
         if mode == "sparse":
             self._step.run()
             y = self.o_s
+        elif mode == "paged":
+            cache.append(self.k_s, self.v_s)
+            y = cache.attend(self.q_s, self.o_s, self.workspace)
         elif x.is_cuda:
             from flash_attn import flash_attn_with_kvcache       # split-KV dense decode (library kernel)
             y = flash_attn_with_kvcache(self.q_s.view(B, 1, self.n_head, self.head_dim),
@@ -356,6 +370,8 @@ class Transformer(Decoder):
         self.norm = RMSNorm(config.dim, eps=config.norm_eps)
         self.output = nn.Linear(config.dim, config.vocab_size, bias=False)
         self.register_buffer("freqs_cis", None, persistent=False)
+        self.paging: Optional[Paging] = None
+        self.pages: Optional[PageTable] = None
         self.tp_fused = True                       # decode: fuse wo / w2 with the sum over the ranks (GPU, <= 8 rows)
         self._fused_sum = None
 
@@ -392,27 +408,64 @@ class Transformer(Decoder):
                 raise ValueError(f"{name}: {tuple(tensors[name].shape)} in the checkpoint, {tuple(dst.shape)} in the model")
             dst.copy_(tensors[name])
 
+    def use_pages(self, paging: Optional[Paging] = Paging()) -> "Transformer":
+        """Keep the caches in pages (None: in one piece per sequence again) and decode with mode "paged".  Caches that are
+        there are dropped: `setup_caches` and `setup_decode` follow."""
+        self.paging, self.pages = paging, None
+        self.default_mode = type(self).default_mode if paging is None else "paged"
+        self.release_decode()
+        self.max_batch_size = self.max_seq_length = -1
+        for layer in self.layers:
+            layer.attention.kv_cache = layer.attention.workspace = None
+        return self
+
+    def choose_mode(self, mode: Optional[str]) -> None:
+        if mode is not None and (mode == "paged") != (self.paging is not None):
+            self.use_pages(Paging() if mode == "paged" else None)
+
     def _alloc_caches(self, batch: int, length: int) -> None:
         """Per-layer caches (K, V, bucket codes, value norms) and the rotary table; as
         GPT-FAST/model.py:251-278 minus the T x T mask."""
+        if self.paging is not None:
+            p = self.paging
+            self.pages = PageTable(batch, length, p.page, p.pages, self.device)
+        for b in self.layers if self.paging is not None else ():
+            a = b.attention
+            a.kv_cache = PagedKVCache(self.pages, a.n_local_heads, a.head_dim, dtype=self.dtype, device=self.device, collect=p.budget > 0)
+        self.freqs_cis = precompute_freqs_cis(min(self.config.block_size, length), self.config.head_dim,
+                                              self.config.rope_base, device=self.device)
+        if self.paging is not None:
+            return
         for b in self.layers:
             a = b.attention
             a.kv_cache = KVCache(batch, length, a.n_local_heads, a.head_dim, L=a.L, R=a.R, dtype=self.dtype,
                                  device=self.device)
-        self.freqs_cis = precompute_freqs_cis(min(self.config.block_size, length), self.config.head_dim,
-                                              self.config.rope_base, device=self.device)
 
     # ------------------------------------------------------------------------------- prefill
     def _portion(self, idx: Tensor, start: int) -> Tensor:
         """Each portion's keys are appended to the caches (hashed on the tensor cores) and its queries
         attend causally over everything cached so far."""
         end = start + idx.shape[1]
+        if self.pages is not None:
+            self._continue_pages(idx.shape[0], start)
+            self.pages.reserve(self.pages.length + idx.shape[1])
         pos = torch.arange(start, end, device=idx.device)
         x = self.tok_embeddings(idx)
         fc = self.freqs_cis[start:end]
         for layer in self.layers:
             x = layer.prefill(x, fc, pos, start)
+        if self.pages is not None:
+            self.pages.advance(idx.shape[1])
         return x
+
+    def _continue_pages(self, batch: int, position: int) -> None:
+        """Caches in pages only grow: a call starts anew at position 0 or goes on where the last one ended."""
+        if batch != self.pages.table.shape[0]:
+            raise RuntimeError(f"{batch} sequences on caches in pages for {self.pages.table.shape[0]}")
+        if position == 0:
+            self.pages.reset()
+        elif position != self.pages.position:
+            raise RuntimeError(f"position {position} on caches in pages that end at {self.pages.position}")
 
     def _head(self, hidden: Tensor) -> Tensor:
         return self.output(self.norm(hidden))
@@ -423,12 +476,64 @@ class Transformer(Decoder):
         fc = None if x.is_cuda else self.freqs_cis[self._pos]   # [1,D/2,2]
         for layer in self.layers:
             x = layer.decode(x, fc, self._pos, self._seqlens, mode, self.freqs_cis)
+        if self.pages is not None:
+            self.pages.counters.add_(1)
         if few_rows_here(x, 1):                                 # every rank holds the whole vocabulary projection
             return project_rows(norm_rows(self.norm, x), self.output)[:, -1]
         return self.output(self.norm(x))[:, -1]
 
+    def setup_decode(self, batch: int, mode: Optional[str] = None, use_graph: bool = True) -> None:
+        if self.pages is None:
+            return super().setup_decode(batch, mode, use_graph)
+        if batch != self.pages.table.shape[0]:
+            raise RuntimeError(f"{batch} sequences on caches in pages for {self.pages.table.shape[0]}")
+        counters = self.pages.counters.clone()
+        flags = [layer.attention.kv_cache.status.clone() for layer in self.layers]
+        self.pages.hide()                                       # the dry run finds no page to write to
+        try:
+            super().setup_decode(batch, mode, use_graph)
+        finally:
+            self.pages.show()
+            self.pages.counters.copy_(counters)
+            for layer, flag in zip(self.layers, flags):
+                layer.attention.kv_cache.status.copy_(flag)
+
+    def start_decode(self, first_token: Tensor, position: int) -> None:
+        if self.pages is not None:
+            self._continue_pages(first_token.shape[0], position)
+        super().start_decode(first_token, position)
+
+    def decode_one_token(self) -> Tensor:
+        if self.pages is None:
+            return super().decode_one_token()
+        if self._host_pos < self.max_seq_length:                # else the call below says so
+            self.pages.reserve(self.pages.length + 1)
+        tok = super().decode_one_token()
+        self.pages.advance(1, on_device=False)
+        p = self.paging
+        if p.budget and self.pages.length >= p.budget + p.every:
+            self.evict(p.budget, p.recent, p.sink)
+        return tok
+
+    @torch.no_grad()
+    def evict(self, budget: int, recent: int = 0, sink: int = 0) -> None:
+        """Cuts every sequence's caches to `budget` slots, in every layer and key/value head by the weight its keys collected."""
+        if self.pages is None or self.layers[0].attention.kv_cache.mass is None:
+            raise RuntimeError("eviction needs caches in pages with a budget: see use_pages")
+        lengths = torch.empty_like(self.pages.lengths)
+        for layer in self.layers:
+            layer.attention.kv_cache.evict(budget, recent, sink, lengths)
+        self.pages.lengths.copy_(lengths)
+        self.pages.cut(min(self.pages.length, budget))
+
     def _setup_decode_layers(self, batch: int, mode: str) -> None:
         dev = self.device
+        if self.pages is not None and dev.type == "cuda":
+            a = self.layers[0].attention
+            need = a.kv_cache.attend_workspace(a.n_head)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            for layer in self.layers:
+                layer.attention.workspace = workspace
         for layer in self.layers:
             layer.attention.setup_decode(batch, self._pos, mode)
         if self.world > 1 and dev.type == "cuda" and self.tp_fused and batch <= 8 and \

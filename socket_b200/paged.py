@@ -11,9 +11,11 @@ Nothing here synchronises with the host, and nothing has a CPU path.
 from __future__ import annotations
 
 import struct
-from typing import Optional, Tuple
+from dataclasses import dataclass
+from typing import List, Optional, Tuple
 
 import torch
+import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
@@ -139,3 +141,123 @@ def evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass
     on_device(index, check, entry.sk_paged_evict, "sk_paged_evict", c, budget, recent, sink, m.data_ptr(), mb, mh, q.data_ptr(), pb, ph,
               n.data_ptr(), ptr(ws), need)
     return out
+
+
+# ---------------------------------------------------------------------------------- caches of a decoder
+@dataclass(frozen=True)
+class Paging:
+    """How a decoder keeps its caches in pages.  With a budget, sequences that have grown `every` tokens beyond it are cut back to
+    it: the first `sink` tokens, the last `recent` ones and the keys that decoded tokens attended to most stay."""
+    page: int = 64
+    pages: int = 0                      # of the pool; 0: as many as all sequences need at their longest
+    budget: int = 0                     # 0: nothing is evicted
+    recent: int = 0
+    sink: int = 0
+    every: int = 64
+
+    def __post_init__(self):
+        if self.page < 16 or self.page & (self.page - 1):
+            raise ValueError(f"pages of {self.page} rows: a power of two, at least 16")
+        if self.budget < 0 or self.recent < 0 or self.sink < 0 or self.pages < 0 or (self.budget and self.recent + self.sink > self.budget):
+            raise ValueError(f"a budget of {self.budget} for {self.sink} first and {self.recent} last tokens, {self.pages} pages")
+        if self.budget and self.every < 1:
+            raise ValueError("evictions need at least one token between them")
+
+
+class PageTable:
+    """Which pages a decoder's sequences hold, the same in every layer: all sequences grow in step.  The host decides, the device
+    reads `table`, `lengths` and `positions` (of the next token)."""
+
+    def __init__(self, batch: int, max_length: int, page: int, pages: int = 0, device=None):
+        self.page, self.width = page, -(-max_length // page)
+        self.pages = pages or batch * self.width
+        self.table = torch.full((batch, self.width), -1, dtype=torch.int32, device=device)
+        self.counters = torch.zeros(2, batch, dtype=torch.int32, device=device)
+        self.lengths, self.positions = self.counters[0], self.counters[1]
+        self.reset()
+
+    def reset(self) -> None:
+        """No tokens, all pages free."""
+        self.free = list(range(self.pages - 1, -1, -1))
+        self.held: List[List[int]] = [[] for _ in range(self.table.shape[0])]
+        self.length = self.position = 0
+        self.counters.zero_()
+        self._show()
+
+    def _show(self) -> None:
+        rows = [held + [-1] * (self.width - len(held)) for held in self.held]
+        self.table.copy_(torch.tensor(rows, dtype=torch.int32).view(self.table.shape))
+
+    def hide(self) -> None:
+        """The device sees no pages until `show`: calls on the cache then write and read nothing."""
+        self.table.fill_(-1)
+
+    show = _show
+
+    def reserve(self, length: int) -> None:
+        """Pages for `length` slots of every sequence."""
+        want = -(-length // self.page)
+        if want > self.width:
+            raise RuntimeError(f"{length} slots in a cache of {self.width * self.page}")
+        if all(len(held) >= want for held in self.held):
+            return
+        if sum(max(0, want - len(held)) for held in self.held) > len(self.free):
+            raise RuntimeError(f"out of pages: {len(self.free)} of {self.pages} free, sequences of {length} slots asked for")
+        for held in self.held:
+            while len(held) < want:
+                held.append(self.free.pop())
+        self._show()
+
+    def cut(self, length: int) -> None:
+        """Slots from `length` on are given back; the device's lengths are the caller's."""
+        keep = -(-length // self.page)
+        for held in self.held:
+            self.free += reversed(held[keep:])
+            del held[keep:]
+        self.length = length
+        self._show()
+
+    def advance(self, tokens: int, on_device: bool = True) -> None:
+        """`tokens` more of every sequence are cached.  Without `on_device` the device has counted them itself."""
+        self.length += tokens
+        self.position += tokens
+        if on_device:
+            self.counters.add_(tokens)
+
+
+class PagedKVCache(nn.Module):
+    """One layer's keys and values in pages, with what eviction goes by."""
+
+    def __init__(self, pages: PageTable, n_heads: int, head_dim: int, dtype=torch.bfloat16, device=None, collect: bool = False):
+        super().__init__()
+        self.pages = pages
+        shape = (pages.pages, n_heads, pages.page, head_dim)
+        self.register_buffer("k_pages", torch.zeros(shape, dtype=dtype, device=device))
+        self.register_buffer("v_pages", torch.zeros(shape, dtype=dtype, device=device))
+        book = (pages.table.shape[0], n_heads, pages.width * pages.page)
+        self.register_buffer("mass", torch.zeros(book, dtype=torch.float32, device=device) if collect else None)
+        self.register_buffer("slot_positions", torch.zeros(book, dtype=torch.int32, device=device) if collect else None)
+        self.register_buffer("status", torch.zeros((), dtype=torch.int32, device=device))
+
+    def append(self, k: Tensor, v: Tensor) -> None:
+        """k, v [B, S, heads, D] behind the cached tokens; `pages.advance` follows once every layer has appended."""
+        append(k, v, self.k_pages, self.v_pages, self.pages.table, self.pages.lengths, first=self.pages.positions,
+               positions=self.slot_positions, mass=self.mass, status=self.status)
+
+    def attend(self, q: Tensor, out: Tensor, workspace: Optional[Tensor] = None) -> Tensor:
+        """q [B, H, D] of the token just appended over everything cached."""
+        return attn(q, self.k_pages, self.v_pages, self.pages.table, self.pages.lengths, extra=1, mass=self.mass, out=out,
+                    workspace=workspace, status=self.status)
+
+    def attend_workspace(self, n_head: int) -> int:
+        return attn_workspace(n_head, self.k_pages, self.v_pages, self.pages.table, self.pages.lengths, mass=self.mass)
+
+    def evict(self, budget: int, recent: int, sink: int, lengths: Tensor) -> None:
+        """Down to `budget` slots; `lengths` gets the new lengths, those of the table stay for the other layers."""
+        evict(self.k_pages, self.v_pages, self.pages.table, self.pages.lengths, self.mass, self.slot_positions, budget=budget, recent=recent,
+              sink=sink, out=(self.mass, self.slot_positions, lengths), status=self.status)
+
+    def rows(self, length: int) -> Tuple[Tensor, Tensor]:
+        """Keys and values [B, heads, length, D] of the first slots, copied out of the pages."""
+        at = self.pages.table[:, :-(-length // self.pages.page)].long()
+        return tuple(pool[at].transpose(1, 2).flatten(2, 3)[:, :, :length] for pool in (self.k_pages, self.v_pages))

@@ -106,3 +106,37 @@ def test_cpu_tensors_are_refused():
         paged.evict(k, k, table, n, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64, dtype=torch.int32), budget=8)
     with pytest.raises(RuntimeError, match="CUDA"):
         few_rows.token_logprobs(torch.zeros(2, 10))
+
+
+def test_page_tables_hand_out_and_take_back_pages():
+    t = paged.PageTable(2, 100, 16, 9)
+    assert t.width == 7 and t.table.tolist() == [[-1] * 7] * 2
+    t.reserve(33)
+    held = [x[:3] for x in t.table.tolist()]
+    assert sorted(held[0] + held[1]) == list(range(6)) and all(x[3:] == [-1] * 4 for x in t.table.tolist()) and len(t.free) == 3
+    t.reserve(48)                                             # still three pages each
+    assert [x[:3] for x in t.table.tolist()] == held
+    t.advance(48)
+    assert t.lengths.tolist() == t.positions.tolist() == [48, 48] and t.length == t.position == 48
+    with pytest.raises(RuntimeError, match="out of pages"):
+        t.reserve(81)                                         # six pages each
+    assert [x[:3] for x in t.table.tolist()] == held and len(t.free) == 3
+    with pytest.raises(RuntimeError, match="113 slots"):
+        t.reserve(113)
+    t.hide()
+    assert (t.table == -1).all()
+    t.show()
+    t.cut(17)
+    assert t.length == 17 and t.position == 48 and [x[:2] for x in t.table.tolist()] == [x[:2] for x in held] and len(t.free) == 5
+    t.reserve(64)
+    pages = [p for x in t.table.tolist() for p in x if p >= 0]
+    assert len(pages) == len(set(pages)) == 8
+    t.reset()
+    assert len(t.free) == 9 and t.lengths.tolist() == [0, 0] and (t.table == -1).all()
+
+
+@pytest.mark.parametrize("over", [dict(page=8), dict(page=48), dict(budget=-1), dict(budget=10, recent=8, sink=3), dict(pages=-1),
+                                  dict(budget=10, every=0), dict(recent=-1)])
+def test_paging_that_is_refused(over):
+    with pytest.raises(ValueError):
+        paged.Paging(**over)
