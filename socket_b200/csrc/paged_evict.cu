@@ -89,7 +89,7 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         uint32_t* keys = ev_raw;
         int32_t* places = reinterpret_cast<int32_t*>(ev_raw + room);
         int newest = INT32_MIN;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = t; i < count; i += EV_THREADS) {
             const int p = pos[j0 + i];
             newest = max(newest, p);
@@ -230,26 +230,35 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         if (rank == 0 && t == 0) rows[row] = EvRow{all_movers, kept};
         EvMove* list = moves + (int64_t)row * most_moves;
         seen = equal_at;
-#pragma unroll 2
-        for (int i = i0 + lane; i - lane < i1; i += 32) {
-            const int j = j0 + i;
-            const float m = i < i1 ? mass[j] : 0.f;
-            const int p = i < i1 ? (HELD ? places[i] : pos[j]) : 0;
-            const bool keep = keeps(i, seen), hole = i < i1 && !keep && i < low, mover = keep && i >= low;
-            const unsigned h = __ballot_sync(FULL, hole), v = __ballot_sync(FULL, mover);
-            if (hole) list[hole_at + __popc(h & ((1u << lane) - 1))].to = j;
-            if (mover) {
-                EvMove* e = list + mover_at + __popc(v & ((1u << lane) - 1));
-                e->from = j;
-                e->mass = m;
-                e->pos = p;
+        constexpr int STEPS = 4;                               // whose masses are asked for at a time
+        for (int first = i0; first < i1; first += 32 * STEPS) {
+            float m[STEPS];
+            int p[STEPS];
+#pragma unroll
+            for (int u = 0; u < STEPS; ++u) {
+                const int i = first + u * 32 + lane;
+                m[u] = i < i1 ? mass[j0 + i] : 0.f;
+                p[u] = i < i1 ? (HELD ? places[i] : pos[j0 + i]) : 0;
             }
-            if (i < i1 && !hole) {                             // a hole's are written with the move
-                mo[j] = i < low ? m : 0.f;
-                po[j] = i < low ? p : -1;
+#pragma unroll
+            for (int u = 0; u < STEPS; ++u) {
+                const int i = first + u * 32 + lane, j = j0 + i;
+                const bool keep = keeps(i, seen), hole = i < i1 && !keep && i < low, mover = keep && i >= low;
+                const unsigned h = __ballot_sync(FULL, hole), v = __ballot_sync(FULL, mover);
+                if (hole) list[hole_at + __popc(h & ((1u << lane) - 1))].to = j;
+                if (mover) {
+                    EvMove* e = list + mover_at + __popc(v & ((1u << lane) - 1));
+                    e->from = j;
+                    e->mass = m[u];
+                    e->pos = p[u];
+                }
+                if (i < i1 && !hole) {                         // a hole's are written with the move
+                    mo[j] = i < low ? m[u] : 0.f;
+                    po[j] = i < low ? p[u] : -1;
+                }
+                hole_at += __popc(h);
+                mover_at += __popc(v);
             }
-            hole_at += __popc(h);
-            mover_at += __popc(v);
         }
     };
     if (share <= room) select(std::true_type{});
