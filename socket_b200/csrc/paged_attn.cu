@@ -132,13 +132,30 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
     auto slots_of = [](int n) { return n == 0 ? 0 : (n + CHUNK - 1) / CHUNK + PT_PAD; };
 
     // ---- this block's run of chunks
-    int64_t total = 0;
-    for (int b = t; b < c.B; b += S::THREADS) {
-        bool over;
-        total += slots_of(paged_length(c, b, a.extra, &over));
-        if (over && blockIdx.x == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
+    int64_t total, before = 0;
+    PtPlace cur;
+    const bool few = c.B <= 32;                                // a lane per sequence, every warp by itself
+    int n_lane = 0;
+    if (few) {
+        bool over = false;
+        n_lane = lane < c.B ? paged_length(c, lane, a.extra, &over) : 0;
+        if (over && blockIdx.x == 0 && warp == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
+        before = slots_of(n_lane);                             // up to this lane's sequence, with it
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(FULL, before, o);
+            if (lane >= o) before += x;
+        }
+        total = __shfl_sync(FULL, before, 31) * units;
+    } else {
+        total = 0;
+        for (int b = t; b < c.B; b += S::THREADS) {
+            bool over;
+            total += slots_of(paged_length(c, b, a.extra, &over));
+            if (over && blockIdx.x == 0 && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
+        }
+        total = pt_block_sum(total, red) * units;
     }
-    total = pt_block_sum(total, red) * units;
     for (int b = blockIdx.x; b < c.B; b += gridDim.x)          // no key, no run: zeros
         if (paged_length(c, b, a.extra) == 0)
             for (int i = t; i < a.H * c.D; i += S::THREADS) ((T*)a.out)[b * a.o_bs + i / c.D * a.o_hs + i % c.D] = from_f32<T>(0.f);
@@ -150,32 +167,37 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
         run->tail_last = -1;
     }
     if (left == 0) return;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < c.B; b0 += S::THREADS) {             // the sequence that holds chunk `first`
-        const int b = b0 + t, n = b < c.B ? paged_length(c, b, a.extra) : 0, m = slots_of(n);
-        int64_t sum = m;
+    auto place = [&](int b, int n, int64_t lo) {               // of chunk `first` in sequence b, whose chunks begin at lo
+        const int m = slots_of(n), unit = (int)((first - lo) / m);
+        return PtPlace{b, unit / a.groups, unit % a.groups, (int)((first - lo) % m), m - PT_PAD, n};
+    };
+    if (few) {
+        const int b = __ffs(__ballot_sync(FULL, before * units > first)) - 1, n = __shfl_sync(FULL, n_lane, b);
+        cur = place(b, n, (__shfl_sync(FULL, before, b) - slots_of(n)) * units);
+    } else {
+        for (int b0 = 0; b0 < c.B; b0 += S::THREADS) {         // the sequence that holds chunk `first`
+            const int b = b0 + t, n = b < c.B ? paged_length(c, b, a.extra) : 0, m = slots_of(n);
+            int64_t sum = m;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(FULL, sum, o);
-            if (lane >= o) sum += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t x = __shfl_up_sync(FULL, sum, o);
+                if (lane >= o) sum += x;
+            }
+            if (lane == 31) red[warp] = sum;
+            __syncthreads();
+            int64_t all = 0;
+            for (int w = 0; w < WARPS; ++w) {
+                if (w < warp) sum += red[w];
+                all += red[w];
+            }
+            const int64_t lo = (before + sum - m) * units, hi = (before + sum) * units;
+            if (lo <= first && first < hi) start_s = place(b, n, lo);
+            before += all;
+            __syncthreads();
+            if (before * units > first) break;
         }
-        if (lane == 31) red[warp] = sum;
-        __syncthreads();
-        int64_t all = 0;
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) sum += red[w];
-            all += red[w];
-        }
-        const int64_t lo = (before + sum - m) * units, hi = (before + sum) * units;
-        if (lo <= first && first < hi) {
-            const int unit = (int)((first - lo) / m);
-            start_s = PtPlace{b, unit / a.groups, unit % a.groups, (int)((first - lo) % m), m - PT_PAD, n};
-        }
-        before += all;
-        __syncthreads();
-        if (before * units > first) break;
+        cur = start_s;
     }
-    PtPlace cur = start_s;
     int64_t flat = first;                                      // chunk in the row of all chunks
     if (cur.chunk >= cur.chunks) {                             // the run begins behind a pair
         const int skip = cur.chunks + PT_PAD - cur.chunk;
@@ -559,34 +581,48 @@ template <typename S> __device__ __forceinline__ const float* pt_part(const PtAr
     return a.parts + ((int64_t)x * 2 + (begins_inside ? 1 : 0)) * S::HG * (S::DP + 2);
 }
 
-// A pair that ends in another run than it begins in belongs to the run it begins in; a run has one such pair at most.  The first HG
-// blocks of a run (blockIdx.x) join its partial results, one head each, a warp every eighth of them; the others, with mass, add the
-// weights of a share of the run's keys.
+// A pair that ends in another run than it begins in belongs to the run it begins in; a run has one such pair at most.  With mass, the
+// warps of the first `shares` blocks of a run (blockIdx.x) add the weights of a share of the run's keys each; the other blocks join the
+// pair's partial results, one head each, a warp every eighth of them.
 constexpr int PJ_WARPS = 8, PJ_SHARES = 4;
 template <typename S, typename T>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
-paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constant__ PtArgs a) {
+paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constant__ PtArgs a, int shares) {
     pdl_begin();
     constexpr int DP = S::DP, HG = S::HG, E = DP / 32, CHUNK = S::CHUNK;
-    __shared__ float ms[PJ_WARPS], ls[PJ_WARPS], os[PJ_WARPS][DP], stat[2][HG];
+    __shared__ float ms[PJ_WARPS], ls[PJ_WARPS], os[PJ_WARPS][DP], stats[PJ_WARPS][2][HG];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, rep = a.H / c.G, x0 = blockIdx.x;
     PtRun run;
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(PtRun) / 16); ++i) reinterpret_cast<int4*>(&run)[i] = __ldcg(reinterpret_cast<const int4*>(a.runs + x0) + i);
-    if (blockIdx.y < HG) {
-        const int last = run.tail_last, h = blockIdx.y, b = run.tail_b, g = run.tail_g, hh = run.tail_grp * HG + h;
+    if ((int)blockIdx.y >= shares) {
+        const int last = run.tail_last, h = blockIdx.y - shares, b = run.tail_b, g = run.tail_g, hh = run.tail_grp * HG + h;
         if (last < 0 || hh >= rep) return;
         float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.f;
-        for (int x = x0 + warp; x <= last; x += PJ_WARPS) {
-            const float* part = pt_part<S>(a, x, x == x0 && run.tail_inside);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + HG * DP + h * 2));
-            const float mn = fmaxf(m, ml.x), f = pt_factor(m, mn), fx = pt_factor(ml.x, mn);
+        constexpr int AHEAD = 3;                               // partial results asked for at a time: up to 24 of a pair in one trip
+        for (int x = x0 + warp; x <= last; x += AHEAD * PJ_WARPS) {
+            float2 ml[AHEAD];
+            float v[AHEAD][E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(__ldcg(part + h * DP + e * 32 + lane), fx, o[e] * f);
-            l = fmaf(ml.y, fx, l * f);
-            m = mn;
+            for (int i = 0; i < AHEAD; ++i) {
+                ml[i] = make_float2(-INFINITY, 0.f);
+                if (x + i * PJ_WARPS > last) continue;
+                const float* part = pt_part<S>(a, x + i * PJ_WARPS, i == 0 && x == x0 && run.tail_inside);
+                ml[i] = __ldcg(reinterpret_cast<const float2*>(part + HG * DP + h * 2));
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[i][e] = __ldcg(part + h * DP + e * 32 + lane);
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (x + i * PJ_WARPS > last) continue;
+                const float mn = fmaxf(m, ml[i].x), f = pt_factor(m, mn), fx = pt_factor(ml[i].x, mn);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fmaf(v[i][e], fx, o[e] * f);
+                l = fmaf(ml[i].y, fx, l * f);
+                m = mn;
+            }
         }
         if (lane == 0) {
             ms[warp] = m;
@@ -611,9 +647,11 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
         }
         return;
     }
-    // ---- mass: pairs and heads of one key/value head add to the same keys; a block adds what all heads of a group weigh, so more
-    // than one group takes turns: units of a key/value head stand one behind the other, and only the first one's chunks are walked
-    const int share = blockIdx.y - HG, from = (int)((int64_t)run.left * share / PJ_SHARES), to = (int)((int64_t)run.left * (share + 1) / PJ_SHARES);
+    // ---- mass: all groups of a key/value head add to the same keys.  Their chunks stand one behind the other, and who walks the first
+    // group's adds for all of them
+    const int share = blockIdx.y * PJ_WARPS + warp, of = PJ_SHARES * PJ_WARPS;
+    const int from = (int)((int64_t)run.left * share / of), to = (int)((int64_t)run.left * (share + 1) / of);
+    float (*stat)[HG] = stats[warp];
     const int64_t per = run.per;
     PtPlace p = {run.b, run.g, run.grp, run.chunk, run.chunks, run.n};
     int64_t flat = run.first;
@@ -627,14 +665,15 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                 const int heads = min(HG, rep - grp * HG);
                 const int64_t begin = flat - p.chunk + (int64_t)grp * (p.chunks + PT_PAD);
                 const int y0 = (int)(begin / per), y1 = (int)((begin + p.chunks - 1) / per);
-                __syncthreads();
-                for (int h = warp; h < heads; h += PJ_WARPS) { // final maximum and 1 / sum
-                    float m = -INFINITY, l = 0.f;
-                    if (y0 == y1) {
-                        const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)p.b * a.H + g * rep + grp * HG + h) * 2));
-                        m = st.x;
-                        l = st.y;
-                    } else {
+                __syncwarp();
+                if (y0 == y1 && lane < heads) {                // final maximum and 1 / sum: there already
+                    const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)p.b * a.H + g * rep + grp * HG + lane) * 2));
+                    stat[0][lane] = st.x == -INFINITY ? 0.f : st.x;
+                    stat[1][lane] = st.y;
+                }
+                if (y0 != y1)
+                    for (int h = 0; h < heads; ++h) {
+                        float m = -INFINITY, l = 0.f;
                         for (int x = y0 + lane; x <= y1; x += 32) {
                             const float2 ml = __ldcg(reinterpret_cast<const float2*>(pt_part<S>(a, x, begin > x * per) + HG * DP + h * 2));
                             const float mn = fmaxf(m, ml.x);
@@ -647,30 +686,38 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                             l = l * pt_factor(m, mn) + l2 * pt_factor(m2, mn);
                             m = mn;
                         }
-                        l = pt_inverse(l);
+                        if (lane == 0) {
+                            stat[0][h] = m == -INFINITY ? 0.f : m;
+                            stat[1][h] = pt_inverse(l);
+                        }
                     }
-                    if (lane == 0) {
-                        stat[0][h] = m == -INFINITY ? 0.f : m;
-                        stat[1][h] = l;
-                    }
-                }
-                __syncthreads();
+                __syncwarp();
                 const float* sc = a.scores + begin * CHUNK * a.rs;
                 if (a.rs == 4) {
                     const float4 m4 = make_float4(stat[0][0], stat[0][1], stat[0][2], stat[0][3]);
                     const float4 l4 = make_float4(stat[1][0], stat[1][1], stat[1][2], heads > 3 ? stat[1][3] : 0.f);
-#pragma unroll 4
-                    for (int j = j0 + t; j < j1; j += PJ_WARPS * 32) {
-                        const float4 x = __ldcs(reinterpret_cast<const float4*>(sc) + j);
-                        float w = exp2_fast(x.x - m4.x) * l4.x;
-                        w = fmaf(exp2_fast(x.y - m4.y), l4.y, w);
-                        w = fmaf(exp2_fast(x.z - m4.z), l4.z, w);
-                        if (heads > 3) w = fmaf(exp2_fast(x.w - m4.w), l4.w, w);
-                        mass[j] += w;
+                    for (int j = j0 + lane; j < j1; j += 128) {
+                        float4 x[4];
+                        float w[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (j + u * 32 < j1) {
+                                x[u] = __ldcs(reinterpret_cast<const float4*>(sc) + j + u * 32);
+                                w[u] = mass[j + u * 32];
+                            }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (j + u * 32 < j1) {
+                                float s = exp2_fast(x[u].x - m4.x) * l4.x;
+                                s = fmaf(exp2_fast(x[u].y - m4.y), l4.y, s);
+                                s = fmaf(exp2_fast(x[u].z - m4.z), l4.z, s);
+                                if (heads > 3) s = fmaf(exp2_fast(x[u].w - m4.w), l4.w, s);
+                                mass[j + u * 32] = w[u] + s;
+                            }
                     }
                 } else {
 #pragma unroll 2
-                    for (int j = j0 + t; j < j1; j += PJ_WARPS * 32) {
+                    for (int j = j0 + lane; j < j1; j += 32) {
                         float w = 0.f;
                         for (int h = 0; h < heads; ++h) w = fmaf(exp2_fast(__ldcg(sc + (int64_t)j * a.rs + h) - stat[0][h]), stat[1][h], w);
                         mass[j] += w;
@@ -760,8 +807,8 @@ int launch_paged_attn(const sk_paged_cache& c, const void* q, int64_t q_bs, int6
         if (e == cudaSuccess) e = launch_after(paged_attn_kernel<S, T>, dim3(p.blocks), dim3(S::THREADS), S::SMEM, st, c, a);
         if (int rc = check_chained(e, "paged_attn_kernel")) return rc;
         if (!p.join) return SK_OK;
-        const dim3 grid(p.blocks, S::HG + (c.mass != nullptr ? PJ_SHARES : 0));
-        return check_chained(launch_after(paged_join_kernel<S, T>, grid, dim3(PJ_WARPS * 32), 0, st, c, a), "paged_join_kernel");
+        const int shares = c.mass != nullptr ? PJ_SHARES : 0, heads = H / c.G < S::HG ? H / c.G : S::HG;
+        return check_chained(launch_after(paged_join_kernel<S, T>, dim3(p.blocks, shares + heads), dim3(PJ_WARPS * 32), 0, st, c, a, shares), "paged_join_kernel");
     });
 }
 
