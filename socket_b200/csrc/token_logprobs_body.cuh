@@ -17,10 +17,15 @@
 namespace sk {
 namespace {
 
-constexpr int LP_THREADS = 256, LP_PER_SM = 3, LP_VECTORS = 4, LP_TOP = 64;
+// Threads of a block.  Many rows: small ones, seven an SM, whose barriers few warps wait at (2048 rows of 128256 bf16, 8 alternatives: 112 us, 4.7 TB/s;
+// three of 256 threads 132; without alternatives 86 and 98).  In clusters rows are few, and larger blocks leave fewer tiles in a row (8 rows of
+// 128256: 12.5 us, with 128 threads 18).
+template <int CL> constexpr int LP_WORK = CL == 1 ? 28 : 24;    // warps of an SM
+constexpr int LP_CLUSTERED = 256;
+template <int CL> constexpr int LP_THREADS = CL == 1 ? 128 : LP_CLUSTERED;
+constexpr int LP_VECTORS = 4, LP_TOP = 64;
 constexpr int LP_STAGES = 3;                                   // tiles in shared memory: 96 KB on their way to an SM at a time
-constexpr int LP_FEW = LP_TOP + 8;                             // threads that may append from one tile
-constexpr int LP_LONG = LP_TOP + 4;                            // a list longer than top + 4 is cut
+constexpr int LP_FEW = 8, LP_LONG = 4;                         // top + LP_FEW threads may append from one tile; a list longer than top + LP_LONG is cut
 constexpr int LP_RANKED = 384;                                 // the longest list that is cut by counting, pair by pair
 constexpr float LP_SLACK = 5.f, LP_LOG2E = 1.4426950408889634f;
 
@@ -132,17 +137,20 @@ __device__ __forceinline__ void lp_join(LpSums& a, LpSums b) {
     a.zd += b.zd;
 }
 
-struct LpShared {
-    uint4 tiles[LP_STAGES][LP_VECTORS][LP_THREADS];            // a thread's vectors are its own
-    LpPair list[LP_FEW * LP_VECTORS * 8 + LP_LONG], best[LP_TOP];
-    LpPair got[8][LP_TOP];                                     // in a cluster's first block: what each has found
-    LpSums sums[8], parts[LP_THREADS / 32];
-    uint32_t least[LP_THREADS / 32];
+template <int THREADS> struct LpShared {
+    uint4 tiles[LP_STAGES][LP_VECTORS][THREADS];            // a thread's vectors are its own
+    LpPair best[LP_TOP];
+    LpPair got[THREADS == 128 ? 1 : 8][LP_TOP];                                     // in a cluster's first block: what each has found
+    LpSums sums[8], parts[THREADS / 32];
+    uint32_t least[THREADS / 32];
     int n, count;
+    LpPair list[];                                             // of lp_room pairs
 };
+// a list that is not long, and all that the threads of a tile append
+constexpr int lp_room(int top, int of_thread) { return (top + LP_FEW) * of_thread + top + LP_LONG; }
 
 // list[0, n) -> best: its `top` largest, in order (all of them if there are fewer); returns how many.  The whole block calls it, with the list complete
-__device__ __forceinline__ int lp_cut(LpShared& s, int n, int top) {
+template <int THREADS> __device__ __forceinline__ int lp_cut(LpShared<THREADS>& s, int n, int top) {
     const int t = threadIdx.x;
     if (n > LP_RANKED) {                                       // the top-th pair by halving, then what reaches it
         LpPair lo = 0, hi = ~0ull;                             // at least `top` reach lo, fewer reach hi
@@ -152,7 +160,7 @@ __device__ __forceinline__ int lp_cut(LpShared& s, int n, int top) {
             if (t == 0) s.count = 0;
             __syncthreads();
             int c = 0;
-            for (int i = t; i < n; i += LP_THREADS) c += s.list[i] >= mid;
+            for (int i = t; i < n; i += THREADS) c += s.list[i] >= mid;
             c = __reduce_add_sync(FULL, c);
             if ((t & 31) == 0) atomicAdd(&s.count, c);
             __syncthreads();
@@ -164,7 +172,7 @@ __device__ __forceinline__ int lp_cut(LpShared& s, int n, int top) {
         __syncthreads();
         if (t == 0) s.count = 0;
         __syncthreads();
-        for (int i = t; i < n; i += LP_THREADS) {
+        for (int i = t; i < n; i += THREADS) {
             const LpPair p = s.list[i];
             if (p >= lo) s.best[atomicAdd(&s.count, 1)] = p;   // `top` of them: no two pairs are equal
         }
@@ -173,7 +181,7 @@ __device__ __forceinline__ int lp_cut(LpShared& s, int n, int top) {
         if (t < n) s.list[t] = s.best[t];
         __syncthreads();
     }
-    for (int i = t; i < n; i += LP_THREADS) {
+    for (int i = t; i < n; i += THREADS) {
         const LpPair p = s.list[i];
         int above = 0;
         for (int x = 0; x < n; ++x) above += s.list[x] > p;
@@ -184,13 +192,14 @@ __device__ __forceinline__ int lp_cut(LpShared& s, int n, int top) {
 }
 
 template <typename T, int CL>
-__global__ void __launch_bounds__(LP_THREADS, LP_PER_SM)
+__global__ void __launch_bounds__(LP_THREADS<CL>, LP_WORK<CL> * 32 / LP_THREADS<CL>)
 token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* token, int top, float* logprob, float* entropy, float* top_logprob,
                       int64_t* top_token, int32_t* status) {
     pdl_begin();
-    constexpr int V = 16 / sizeof(T), U = LP_VECTORS, TILE = LP_THREADS * U;      // vectors of a tile
+    constexpr int THREADS = LP_THREADS<CL>;
+    constexpr int V = 16 / sizeof(T), U = LP_VECTORS, TILE = THREADS * U;      // vectors of a tile
     extern __shared__ __align__(16) char lp_raw[];
-    LpShared& s = *reinterpret_cast<LpShared*>(lp_raw);
+    LpShared<THREADS>& s = *reinterpret_cast<LpShared<THREADS>*>(lp_raw);
     if (CL > 1) cluster_arrive();
     const int t = threadIdx.x, lane = t & 31, rank = CL > 1 ? blockIdx.x % CL : 0;
     const int64_t r = blockIdx.x / CL;
@@ -211,7 +220,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
         const int at = (i0 + t) * V - skew;
         const T* p = x + at;
         auto take = [&](int u) {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + u * LP_THREADS * V));
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p + u * THREADS * V));
             v[u].w[0] = a.x;
             v[u].w[1] = a.y;
             v[u].w[2] = a.z;
@@ -223,8 +232,8 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int a = at + u * LP_THREADS * V;
-                if (i0 + u * LP_THREADS + t >= end) v[u] = lp_edge(x, vocab, vocab);
+                const int a = at + u * THREADS * V;
+                if (i0 + u * THREADS + t >= end) v[u] = lp_edge(x, vocab, vocab);
                 else if (a >= 0 && a + V <= vocab) take(u);
                 else v[u] = lp_edge(x, a, vocab);
             }
@@ -235,15 +244,15 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
             const int at = (i0 + t) * V - skew;
             if (i0 * V >= skew && i0 + TILE <= end && (i0 + TILE) * V - skew <= vocab) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) cp16(saddr(&s.tiles[stage][u][t]), x + at + u * LP_THREADS * V, true);
+                for (int u = 0; u < U; ++u) cp16(saddr(&s.tiles[stage][u][t]), x + at + u * THREADS * V, true);
             } else {
 #pragma unroll 1
                 for (int u = 0; u < U; ++u) {
-                    const int a = at + u * LP_THREADS * V;
-                    if (i0 + u * LP_THREADS + t < end && a >= 0 && a + V <= vocab) {
+                    const int a = at + u * THREADS * V;
+                    if (i0 + u * THREADS + t < end && a >= 0 && a + V <= vocab) {
                         cp16(saddr(&s.tiles[stage][u][t]), x + a, true);
                     } else {
-                        const Vec v = lp_edge(x, i0 + u * LP_THREADS + t < end ? a : vocab, vocab);
+                        const Vec v = lp_edge(x, i0 + u * THREADS + t < end ? a : vocab, vocab);
                         s.tiles[stage][u][t] = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
                     }
                 }
@@ -253,19 +262,19 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
     };
     // What of a tile reaches `bound` goes to the list, vector by vector of the threads that have some: a lane per element, word(u, k, from)
     // the k-th word of the u-th vector of lane `from`
-    constexpr int ROOM = sizeof(s.list) / sizeof(LpPair);
+    const int room = lp_room(top, U * V);
     auto append = [&](int i0, bool mine, LpPair bound, auto&& word) {
         for (unsigned who = __ballot_sync(FULL, mine); who != 0u; who &= who - 1) {
             const int from = __ffs(who) - 1, u = lane / Vec::WORD / 4 % U, k = lane / Vec::WORD % 4;
             const uint32_t w = word(u, k, from);
-            const int i = i0 + u * LP_THREADS + (t & ~31) + from, at = i * V - skew + k * Vec::WORD + lane % Vec::WORD;
+            const int i = i0 + u * THREADS + (t & ~31) + from, at = i * V - skew + k * Vec::WORD + lane % Vec::WORD;
             const LpPair p = lp_pair(Vec::of(w, lane % Vec::WORD), at);
             const bool in = lane < U * V && i < end && at >= 0 && at < vocab && p >= bound;
             const unsigned all = __ballot_sync(FULL, in);
             int place = 0;
             if (lane == 0 && all != 0u) place = atomicAdd(&s.n, __popc(all));
             place = __shfl_sync(FULL, place, 0) + __popc(all & ((1u << lane) - 1));
-            if (in && place < ROOM) s.list[place] = p;
+            if (in && place < room) s.list[place] = p;
         }
     };
     // a thread's pairs of a tile are at most (its largest logit, its first index); a thread outside the row has key 0
@@ -275,7 +284,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
     };
     // to the list's `top` largest, if it is long; the bound that follows
     auto meet = [&](int n, LpPair bound) {
-        if (n <= top + 4) return bound;
+        if (n <= top + LP_LONG) return bound;
         n = lp_cut(s, n, top);
         if (t < n) s.list[t] = s.best[t];
         if (t == 0) s.n = n;
@@ -292,7 +301,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
         for (int u = 1; u < U; ++u) most = lp_max(most, v[u].largest());
         const uint32_t key = key_of(i0, most);
         const int some = __syncthreads_count(reaches(i0, key, bound));
-        if (some > top + 8) {
+        if (some > top + LP_FEW) {
             uint32_t lo = (uint32_t)(bound >> 32);
             int64_t hi = 1ll << 32;                            // at least `top` reach lo, fewer reach hi
             int n = some;
@@ -302,13 +311,13 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
                 if (c >= top) {
                     lo = mid;
                     n = c;
-                    if (c <= top + 8) break;
+                    if (c <= top + LP_FEW) break;
                 } else {
                     hi = mid;
                 }
             }
             LpPair b = (LpPair)lo << 32;
-            if (n > top + 8 || lo == (uint32_t)(bound >> 32)) {           // many equal maxima: by the index of each thread's first one
+            if (n > top + LP_FEW || lo == (uint32_t)(bound >> 32)) {           // many equal maxima: by the index of each thread's first one
                 const int above = __syncthreads_count(key > lo);
                 int at = INT32_MAX;
                 if (key == lo && lo != 0u) {
@@ -316,7 +325,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
                     for (int u = U - 1; u >= 0; --u)
 #pragma unroll
                         for (int k = V / 2 - 1; k >= 0; --k) {
-                            const int i = i0 + u * LP_THREADS + t, a = i * V - skew + k * 2;
+                            const int i = i0 + u * THREADS + t, a = i * V - skew + k * 2;
                             const float2 e = v[u].two(k);
                             if (i < end && a + 1 >= 0 && a + 1 < vocab && lp_key(e.y) == lo) at = a + 1;
                             if (i < end && a >= 0 && a < vocab && lp_key(e.x) == lo) at = a;
@@ -344,7 +353,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
             return w;
         });
         __syncthreads();
-        return meet(min(s.n, ROOM), bound);
+        return meet(min(s.n, room), bound);
     };
 
     LpSums sum = {-INFINITY, 0.f, 0.f};
@@ -402,7 +411,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
         sum.zd += two[0] + two[1];
         if (top > 0) {
             if (tile == 1) {                                   // an equal share of `top` maxima from each warp inside the row
-                const int warps = min((end - i0) / 32, LP_THREADS / 32), each = warps > 0 ? (top + warps - 1) / warps : 33;
+                const int warps = min((end - i0) / 32, THREADS / 32), each = warps > 0 ? (top + warps - 1) / warps : 33;
                 uint32_t left = key_of(i0, most), least = 0;
                 if (each <= 32 && t >> 5 < warps)
                     for (int i = 0; i < each; ++i) {
@@ -421,7 +430,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
             if ((tile & (tile - 1)) == 0 || tile % 8 == 0 || i0 + TILE >= end) {
                 __syncthreads();
                 const int n = s.n;
-                if (n <= ROOM) {
+                if (n <= room) {
                     bound = meet(n, bound);
                 } else {                                       // too many: those tiles again, with care
                     __syncthreads();
@@ -444,9 +453,9 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
     if (lane == 0) s.parts[t >> 5] = sum;
     __syncthreads();
     const int found = top > 0 ? lp_cut(s, s.n, top) : 0;
-    sum = s.parts[lane % (LP_THREADS / 32)];
+    sum = s.parts[lane % (THREADS / 32)];
 #pragma unroll
-    for (int o = LP_THREADS / 64; o >= 1; o >>= 1)
+    for (int o = THREADS / 64; o >= 1; o >>= 1)
         lp_join(sum, LpSums{__shfl_xor_sync(FULL, sum.m, o), __shfl_xor_sync(FULL, sum.z, o), __shfl_xor_sync(FULL, sum.zd, o)});
     if (CL > 1) {
         cluster_wait();                                        // every block of the cluster has begun
@@ -469,7 +478,7 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
             lp_join(sum, LpSums{__shfl_xor_sync(FULL, sum.m, o), __shfl_xor_sync(FULL, sum.z, o), __shfl_xor_sync(FULL, sum.zd, o)});
         // the rank of a pair among all blocks': how many of each block's sorted list are larger
         if (top > 0) {
-            for (int i = t; i < CL * top; i += LP_THREADS) {
+            for (int i = t; i < CL * top; i += THREADS) {
                 const LpPair p = s.got[i / top][i % top];
                 int above = 0;
                 for (int c = 0; c < CL; ++c) {
@@ -504,8 +513,9 @@ int logprobs_launch(const void* logits, int64_t ld, int64_t rows, int vocab, con
                     float* top_logprob, int64_t* top_token, int32_t* status, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * CL));
-    cfg.blockDim = dim3(LP_THREADS);
-    cfg.dynamicSmemBytes = sizeof(LpShared);
+    cfg.blockDim = dim3(LP_THREADS<CL>);
+    constexpr int OF_THREAD = LP_VECTORS * 16 / (int)sizeof(T);
+    cfg.dynamicSmemBytes = sizeof(LpShared<LP_THREADS<CL>>) + lp_room(top, OF_THREAD) * sizeof(LpPair);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -516,7 +526,7 @@ int logprobs_launch(const void* logits, int64_t ld, int64_t rows, int vocab, con
     cfg.attrs = attr;
     cfg.numAttrs = CL > 1 ? 2 : 1;
     static SmemLimit limit;
-    const cudaError_t e = limit.raise((const void*)token_logprobs_kernel<T, CL>, sizeof(LpShared));
+    const cudaError_t e = limit.raise((const void*)token_logprobs_kernel<T, CL>, sizeof(LpShared<LP_THREADS<CL>>) + lp_room(LP_TOP, OF_THREAD) * sizeof(LpPair));
     if (e != cudaSuccess) return check_chained(e, "token_logprobs_kernel");
     return check_chained(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, CL>, (const T*)logits, ld, vocab, token, top, logprob, entropy,
                                             top_logprob, top_token, status), "token_logprobs_kernel");
@@ -538,8 +548,8 @@ int token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int 
         auto with = [&](auto cl) {
             return logprobs_launch<T, decltype(cl)::value>(logits, ld, rows, vocab, token, top, logprob, entropy, top_logprob, top_token, status, st);
         };
-        // blocks of a row: as long as they find a place at once (LP_PER_SM an SM) and have a tile to walk
-        const int64_t places = (int64_t)sm_count() * LP_PER_SM;
+        // blocks of a row: as long as they find a place at once on the SMs and have a tile to walk
+        const int64_t places = (int64_t)sm_count() * (LP_WORK<8> * 32 / LP_CLUSTERED);
         if (rows * 8 <= places && vocab >= 8 * 2048) return with(std::integral_constant<int, 8>{});
         if (rows * 4 <= places && vocab >= 4 * 2048) return with(std::integral_constant<int, 4>{});
         if (rows * 2 <= places && vocab >= 2 * 2048) return with(std::integral_constant<int, 2>{});
