@@ -144,7 +144,7 @@ int sk_paged_evict(const sk_paged_cache* c, int budget, int recent, int sink, fl
     SK_REQUIRE(budget >= 1 && recent >= 0 && sink >= 0 && (int64_t)recent + sink <= budget, "sk_paged_evict: a budget of %d for %d first and %d last",
                budget, sink, recent);
     if (c->B == 0) return SK_OK;
-    SK_REQUIRE(c->mass && c->positions && mass_out && pos_out && lengths_out, "sk_paged_evict: null pointer");
+    SK_REQUIRE(lengths_out && (c->width == 0 || (c->mass && c->positions && mass_out && pos_out)), "sk_paged_evict: null pointer");
     const size_t need = paged_evict_workspace(*c, budget);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(SK_ERR_WORKSPACE, "sk_paged_evict: workspace of %zu bytes, %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);

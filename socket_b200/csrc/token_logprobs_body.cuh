@@ -2,8 +2,8 @@
 //
 //   Z = sum exp(x - m),  log p_t = x_t - m - log Z,  H = log Z - sum exp(x - m) (x - m) / Z
 //
-// Bound by reading the logits, once: every thread keeps a reference m of its own, raised only for a logit LP_SLACK above it, with the two
-// sums; they are brought to one reference at the end.  Alternatives are (logit, index) pairs as one number, so that equal logits have an
+// Bound by reading the logits, once: every thread keeps a reference m of its own among its logits, raised only for one LP_SLACK above it, with
+// the two sums over its other ones; they are brought to one reference at the end.  Alternatives are (logit, index) pairs as one number, so that equal logits have an
 // order and no two are the same.  A block walks its row in tiles and knows a bound that at least `top` pairs reach.  Threads whose maximum
 // of a tile (it comes with the sums) reaches the bound append what does to a list in shared memory; from time to time the block meets, and
 // cuts a list grown long to its `top` largest, whose last one is the new bound.  The first bound is the least of what `top` maxima of
@@ -110,31 +110,34 @@ __device__ __forceinline__ Lp2 lp_fma(Lp2 a, Lp2 b, Lp2 c) {
     return r;
 }
 
-// sum of exp(x - m), and of that times x - m
+// A reference m, one of the logits; over all the others the sum z of exp(x - m), and of that times x - m.  The logit m itself, whose weight is 1,
+// is left out: where it has nearly all of the probability, 1 + z would keep next to nothing of z, which is what its log probability is made of
 struct LpSums {
     float m, z, zd;
 };
+// to a larger reference, which is not among the sums
 __device__ __forceinline__ void lp_raise(LpSums& s, float m) {
-    if (s.m == -INFINITY) {
-        s.m = m;
-        return;
+    if (s.m != -INFINITY) {
+        const float d = s.m - m, f = exp2_fast(d * LP_LOG2E), all = s.z + 1.f;
+        s.zd = f * fmaf(fmaxf(d, -200.f), all, s.zd);          // below -200 the factor is zero
+        s.z = f * all;
     }
-    const float d = s.m - m, f = exp2_fast(d * LP_LOG2E);
-    s.zd = f * fmaf(fmaxf(d, -200.f), s.z, s.zd);              // below -200 the factor is zero
-    s.z *= f;
     s.m = m;
 }
 __device__ __forceinline__ void lp_join(LpSums& a, LpSums b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) {                                      // sums without a logit above -inf: zeros or NaN
+    if (b.m > a.m) {
+        const LpSums x = a;
+        a = b;
+        b = x;
+    }
+    if (b.m == -INFINITY) {                                    // no logit above -inf: zeros or NaN
         a.z += b.z;
         a.zd += b.zd;
         return;
     }
-    lp_raise(a, m);
-    lp_raise(b, m);
-    a.z += b.z;
-    a.zd += b.zd;
+    const float d = b.m - a.m, f = exp2_fast(d * LP_LOG2E), all = b.z + 1.f;
+    a.zd += f * fmaf(fmaxf(d, -200.f), all, b.zd);
+    a.z = fmaf(f, all, a.z);
 }
 
 template <int THREADS> struct LpShared {
@@ -377,12 +380,14 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
         float most = cur[0].largest();
 #pragma unroll
         for (int u = 1; u < U; ++u) most = lp_max(most, cur[u].largest());
-        if (most > sum.m + LP_SLACK || sum.m == -INFINITY) lp_raise(sum, most == most ? most : sum.m);
+        const bool raise = most > sum.m + LP_SLACK || (sum.m == -INFINITY && most > -INFINITY);
+        if (raise) lp_raise(sum, most);
         const float m = sum.m == -INFINITY ? 0.f : sum.m;
         const Lp2 minus = lp_two(-m, -m), log2e = lp_two(LP_LOG2E, LP_LOG2E);
-        Lp2 z = 0, zd = 0;
+        Lp2 z[U], zd = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            z[u] = 0;
 #pragma unroll
             for (int k = 0; k < V / 2; ++k) {
                 const float2 e = cur[u].two(k);
@@ -390,11 +395,30 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
                 float y[2];
                 lp_split(lp_mul(d, log2e), y[0], y[1]);
                 const Lp2 w = lp_two(exp2_fast(y[0]), exp2_fast(y[1]));
-                z = lp_add(z, w);
+                z[u] = lp_add(z[u], w);
                 zd = lp_fma(w, d, zd);
             }
+        }
+        if (raise) {                                           // the vector of the new reference again, without it
+            bool out = false;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (!out && cur[u].largest() == most) {
+                    float a = 0.f;
+#pragma unroll
+                    for (int k = 0; k < V / 2; ++k) {
+                        const float2 e = cur[u].two(k);
+                        const bool x_out = !out && e.x == most, y_out = !out && !x_out && e.y == most;
+                        a += x_out ? 0.f : exp2_fast((e.x - m) * LP_LOG2E);
+                        a += y_out ? 0.f : exp2_fast((e.y - m) * LP_LOG2E);
+                        out |= x_out || y_out;
+                    }
+                    z[u] = lp_two(a, 0.f);
+                }
+        }
         float two[2];
-        lp_split(z, two[0], two[1]);
+        static_assert(U == 4, "the sum of the vectors' sums");
+        lp_split(lp_add(lp_add(z[0], z[1]), lp_add(z[2], z[3])), two[0], two[1]);
         sum.z += two[0] + two[1];
         lp_split(zd, two[0], two[1]);
         if (two[0] + two[1] != two[0] + two[1]) {              // a logit of -inf: it adds 0, not 0 * -inf
@@ -495,10 +519,13 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
             __syncthreads();
         }
     }
-    // ---- the row's results
-    const float lz = sum.z == 0.f ? NAN : logf(sum.z);         // no logit above -inf: no distribution
+    // ---- the row's results, of one lane's sums: of two equal references either may have become the other's
+    sum.m = __shfl_sync(FULL, sum.m, 0);
+    sum.z = __shfl_sync(FULL, sum.z, 0);
+    sum.zd = __shfl_sync(FULL, sum.zd, 0);
+    const float lz = fabsf(sum.m) == INFINITY ? NAN : log1pf(sum.z);      // no logit above -inf, or one of +inf: no distribution
     if (t == 0) {
-        if (entropy != nullptr) entropy[r] = lz - sum.zd / sum.z;
+        if (entropy != nullptr) entropy[r] = lz - sum.zd / (1.f + sum.z);
         if (token != nullptr) logprob[r] = x_token - sum.m - lz;
     }
     if (t < top) {

@@ -549,7 +549,7 @@ class Transformer(Decoder):
 
     def _release_decode_layers(self) -> None:
         for layer in self.layers:
-            layer.attention._step = None
+            layer.attention._step = layer.attention.workspace = None
             layer.fused_sum = None
 
     def _decode_lengths(self) -> list:

@@ -72,7 +72,8 @@ def append(k_new: Tensor, v_new: Tensor, k_pages: Tensor, v_pages: Tensor, table
            mass: Optional[Tensor] = None, status: Optional[Tensor] = None) -> None:
     """k_new, v_new [B, S, G, D] go to the slots from lengths[b] on: all S tokens, or the first counts[b] (int32) of a padded
     batch.  Their mass starts at 0; their positions are first[b] (int32; without it the slot) and up.  `lengths` stays as it is:
-    the caller adds the counts once every layer has appended.  Pages written belong to one sequence each."""
+    the caller adds the counts once every layer has appended.  Pages written belong to one sequence each; rows of k_new and
+    v_new start on 16-byte boundaries."""
     c = _cache(k_pages, v_pages, table, lengths, mass, positions, status)
     _same_device(k_pages.get_device(), k_new, v_new, counts, first)
     B, S, G, D = k_new.shape
@@ -87,6 +88,9 @@ def append(k_new: Tensor, v_new: Tensor, k_pages: Tensor, v_pages: Tensor, table
 
 def attn_workspace(H: int, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *, mass: Optional[Tensor] = None) -> int:
     """Scratch bytes of `attn` with H query heads on this cache."""
+    if k_pages.get_device() not in (-1, torch.cuda.current_device()):          # sized for the SMs of the cache's device
+        with torch.cuda.device(k_pages.device):
+            return attn_workspace(H, k_pages, v_pages, table, lengths, mass=mass)
     return int(lib().sk_paged_attn_workspace_bytes(_cache(k_pages, v_pages, table, lengths, mass, None, None), H))
 
 
@@ -95,10 +99,13 @@ def attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Te
          status: Optional[Tensor] = None) -> Tensor:
     """q [B, H, D], one new token per sequence, attends to the first lengths[b] + extra slots of its pages -> [B, H, D]; a
     sequence without keys gets zeros.  `scale` defaults to 1 / sqrt(D).  With `mass` every attended slot collects its weight,
-    summed over the query heads of its key/value head.  A workspace that is absent or too small is allocated; calls that may
-    run at the same time need one each."""
+    summed over the query heads of its key/value head.  Rows of q and out start on 16-byte boundaries, as those of the pools do.
+    A workspace that is absent or too small is allocated; calls that may run at the same time need one each."""
     c = _cache(k_pages, v_pages, table, lengths, mass, None, status)
     index = k_pages.get_device()
+    if index != torch.cuda.current_device():                  # the split, and its scratch, go by the device's SMs
+        with torch.cuda.device(index):
+            return attn(q, k_pages, v_pages, table, lengths, extra=extra, scale=scale, mass=mass, out=out, workspace=workspace, status=status)
     _same_device(index, q, out, workspace)
     shape, qs = q.shape, q.stride()
     B, H, D = shape
@@ -127,6 +134,9 @@ def evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass
     eviction in place.  Other tensors must not overlap the inputs, nor one another.  Pages of one sequence are no other's."""
     c = _cache(k_pages, v_pages, table, lengths, mass, positions, status)
     index, dev = k_pages.get_device(), k_pages.device
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return evict(k_pages, v_pages, table, lengths, mass, positions, budget=budget, recent=recent, sink=sink, out=out, status=status)
     B, G, slots = table.shape[0], k_pages.shape[1], table.shape[1] * k_pages.shape[2]
     if out is None:
         out = (torch.empty(B, G, slots, dtype=torch.float32, device=dev), torch.empty(B, G, slots, dtype=torch.int32, device=dev),

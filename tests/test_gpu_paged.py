@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from paged_util import Cache, attend, check_attention, keep, moves
+from tests.paged_util import Cache, attend, check_attention, keep, moves
 from socket_b200 import _lib, paged
 
 pytestmark = pytest.mark.gpu
@@ -76,6 +76,30 @@ def test_attention_of_strided_tensors(dtype):
     paged.attn(q, c.k, c.v, table[:, :c.width], c.lengths, out=out[:, :, 0], mass=m)
     check_attention(out[:, :, 0], m, before, q, c, lengths)
     assert (out[:, :, 1] == 7).all()
+
+
+def test_sequences_without_pages():
+    """A table without columns, a pool without pages, no sequences: nothing to attend to, nothing to move."""
+    k = torch.empty(0, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    table, n = torch.empty(3, 0, dtype=torch.int32, device=DEV), torch.tensor([0, -2, 0], dtype=torch.int32, device=DEV)
+    q, mass, pos = torch.randn(3, 4, 64, device=DEV).bfloat16(), torch.empty(3, 2, 0, device=DEV), torch.empty(3, 2, 0, dtype=torch.int32, device=DEV)
+    flag = _flag()
+    for m in (None, mass):
+        assert (paged.attn(q, k, k, table, n, mass=m, status=flag) == 0).all()
+    assert paged.evict(k, k, table, n, mass, pos, budget=4, status=flag)[2].tolist() == [0, 0, 0] and int(flag) == 0
+    assert (paged.attn(q, k, k, table, n, extra=1, status=flag) == 0).all() and int(flag) == _lib.SK_DEV_POS_OUT_OF_RANGE
+    c = Cache([5], 2, 64, 16, torch.bfloat16, DEV)
+    none = (c.k, c.v, c.table[:0], c.lengths[:0])
+    assert paged.attn(q[:0], *none).shape == (0, 4, 64)
+    paged.append(q[:0, None, :2], q[:0, None, :2], *none)
+    books = torch.empty(0, 2, c.cap, device=DEV), torch.empty(0, 2, c.cap, dtype=torch.int32, device=DEV)
+    assert paged.evict(*none, *books, budget=4)[2].shape == (0,)
+
+
+def test_results_in_place_of_the_queries():
+    c = Cache([3000, 40, 129, 7], 2, 128, 16, torch.bfloat16, DEV)
+    q, out, m, before = _run(c, 8, False)
+    assert paged.attn(q, *c.tensors, out=q) is q and torch.equal(q, out)
 
 
 def test_attention_extra_and_scale():

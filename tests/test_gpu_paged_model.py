@@ -4,12 +4,13 @@ import json
 import pytest
 import torch
 
-from paged_util import attend
+from tests.paged_util import attend
 from socket_b200 import generate as command
 from socket_b200.decoder import generate
 from socket_b200.model import ModelArgs, Transformer
 from socket_b200.paged import Paging
-from socket_b200.registry import write_safetensors
+from socket_b200.registry import build_model, write_safetensors
+from tests.radapel_util import CONFIGS
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -163,6 +164,21 @@ def test_scores_of_a_prompt(paged):
     assert got.logprobs.shape == (3, 89) and (got.logprobs.double() - want).abs().max() <= tol
     assert ((got.entropy.double() + (lp.exp() * lp).sum(-1)).abs() <= 8 * tol).all()
     assert got.top_tokens.shape == (3, 89, 3) and (got.top_logprobs.double() - lp.topk(3).values).abs().max() <= tol
+
+
+def test_scores_of_a_prompt_through_listed_layers():
+    model = build_model(CONFIGS["wide"], None, torch.float32, DEV).init_random(5)
+    prompt = torch.randint(0, CONFIGS["wide"]["vocab"], (2, 70), generator=torch.Generator().manual_seed(1)).to(DEV)
+    model.setup_caches(2, 80)
+    logits = model.forward_portion(prompt, 0, range(70)).double()
+    lp = torch.log_softmax(logits[:, :-1], -1)
+    got = model.score(prompt, top=1, chunk=33)
+    # fp32 products summed in other tiles: a few thousand half steps of the logits' size
+    tol = 4096 * 2.0 ** -24 * (1 + logits.abs().max())
+    assert ((got.logprobs.double() - lp.gather(2, prompt[:, 1:, None])[..., 0]).abs() <= tol).all()
+    assert ((got.entropy.double() + (lp.exp() * lp).sum(-1)).abs() <= 8 * tol).all()
+    seq, stats = generate(model, prompt.cpu(), 5, logprobs=2)
+    assert torch.equal(stats["logprobs"].top_tokens[..., 0], seq[:, 70:])
 
 
 @pytest.mark.parametrize("mode", ["sparse", "dense", "paged"])

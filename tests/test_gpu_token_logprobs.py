@@ -96,6 +96,28 @@ def test_rows_without_a_distribution(vocab):
         assert torch.equal(a[4], b[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [100, 3000, 60000, 128256])
+def test_a_token_that_is_nearly_certain(vocab, dtype):
+    """One logit far above the sum of all others: its log probability is that sum, to a few half steps of itself (terms are exponentials
+    of differences of up to 45, each off by 45 half steps and two of the exponential's; they are summed in a few hundred steps at most)."""
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.randn(12, vocab, generator=g, device=DEV).to(dtype)
+    at = torch.randint(0, vocab, (12,), generator=g, device=DEV)
+    gap = torch.arange(12, device=DEV) * 2.0 + 6 + math.log(vocab)
+    x[torch.arange(12, device=DEV), at] = gap.to(dtype)
+    got = few_rows.token_logprobs(x, at, top=2)
+    y = x.double()
+    d = y - y.gather(1, at[:, None])
+    rest = torch.where(d == 0, 0.0, d.exp()).sum(-1)
+    want = -torch.log1p(rest)
+    assert (want > -0.01).all() and ((got.logprobs.double() - want).abs() <= want.abs() * 600 * 2.0 ** -24).all()
+    p, q = d.exp() / (1 + rest[:, None]), d + want[:, None]
+    entropy = -(p * q).sum(-1)
+    assert ((got.entropy.double() - entropy).abs() <= entropy * 800 * 2.0 ** -24).all()
+    assert torch.equal(got.top_logprobs[:, 0], got.logprobs) and torch.equal(got.top_tokens[:, 0], at)
+
+
 def test_rows_of_other_layouts():
     big = torch.randn(40, 3001, device=DEV).bfloat16()
     tokens = torch.randint(0, 2999, (40,), device=DEV)
