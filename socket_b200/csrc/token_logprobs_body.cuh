@@ -17,9 +17,9 @@
 namespace sk {
 namespace {
 
-// Threads of a block.  Many rows: small ones, seven an SM, whose barriers few warps wait at (2048 rows of 128256 bf16, 8 alternatives: 112 us, 4.7 TB/s;
-// three of 256 threads 132; without alternatives 86 and 98).  In clusters rows are few, and larger blocks leave fewer tiles in a row (8 rows of
-// 128256: 12.5 us, with 128 threads 18).
+// Threads of a block.  Many rows: small ones, seven an SM, whose barriers few warps wait at (2048 rows of 128256 bf16, 8 alternatives: 121 us, 4.3 TB/s,
+// with six an SM 128; without alternatives 92).  In clusters rows are few, and larger blocks leave fewer tiles in a row (8 rows of 128256: 13 us, with
+// 128 threads 18).
 template <int CL> constexpr int LP_WORK = CL == 1 ? 28 : 24;    // warps of an SM
 constexpr int LP_CLUSTERED = 256;
 template <int CL> constexpr int LP_THREADS = CL == 1 ? 128 : LP_CLUSTERED;
