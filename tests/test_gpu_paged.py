@@ -38,6 +38,32 @@ def test_attention(H, G, D, dtype, mass):
     check_attention(out, m, before, q, c, LENGTHS)
 
 
+@pytest.mark.parametrize("D", [4, 12, 100, 132, 252])
+def test_attention_of_fp32_heads_of_odd_sizes(D):
+    c = Cache(LENGTHS, 2, D, 16, torch.float32, DEV, seed=D)
+    q, out, m, before = _run(c, 10, True)
+    check_attention(out, m, before, q, c, LENGTHS)
+
+
+@pytest.mark.parametrize("scale", [-0.7, 0.0, 3.0])
+def test_attention_scales(scale):
+    c = Cache(LENGTHS, 2, 64, 32, torch.float16, DEV)
+    q, out, m, before = _run(c, 6, True, scale=scale)
+    check_attention(out, m, before, q, c, LENGTHS, scale=scale)
+
+
+def test_queries_and_new_rows_that_are_expanded():
+    """One query for every sequence, one new row for every head."""
+    c = Cache([70, 5, 300], 2, 64, 16, torch.bfloat16, DEV, room=3)
+    q = torch.randn(1, 4, 64, device=DEV).bfloat16().expand(3, 4, 64)
+    out = paged.attn(q, *c.tensors)
+    check_attention(out, None, None, q, c, [70, 5, 300])
+    new = torch.randn(3, 1, 1, 64, device=DEV).bfloat16().expand(3, 3, 2, 64)
+    paged.append(new, new, *c.tensors)
+    for b, n in enumerate((70, 5, 300)):
+        assert torch.equal(c.get(c.k, b, n + 3)[:, n:], new[b].transpose(0, 1)) and torch.equal(c.get(c.v, b, n + 3)[:, n:], new[b].transpose(0, 1))
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 512])
 @pytest.mark.parametrize("lengths", [[1], [7, 0, 0, 3], [5000], [0, 0], [3000, 1, 2999, 130, 0, 64]])
 def test_attention_pages(page, lengths):
@@ -348,6 +374,35 @@ def test_evict_layouts(G, D, page, dtype, combined):
 @pytest.mark.parametrize("fill", ["random", "few"])
 def test_evict_long(n, budget, fill):
     _evict_case([n, n // 2], 2, 8, 64, torch.bfloat16, budget, min(100, budget // 2), 1, fill)
+
+
+def test_evictions_captured_and_replayed():
+    """A graph that collects weights and cuts in place, replayed: the same as eager calls on copies."""
+    c = Cache([200, 90, 131], 2, 64, 16, torch.bfloat16, DEV, room=40)
+    q, new = torch.randn(3, 4, 64, device=DEV).bfloat16(), torch.randn(3, 30, 2, 64, device=DEV).bfloat16()
+    mass = torch.rand(3, 2, c.cap, device=DEV)
+    pos = torch.arange(c.cap, dtype=torch.int32, device=DEV).expand(3, 2, c.cap).contiguous()
+
+    def turn(k, v, n, m, p):
+        paged.append(new, new, k, v, c.table, n, positions=p, mass=m)
+        n.add_(30)
+        paged.attn(q, k, v, c.table, n, mass=m)
+        paged.evict(k, v, c.table, n, m, p, budget=100, recent=7, sink=2, out=(m, p, n))
+
+    copies = [t.clone() for t in (c.k, c.v, c.lengths, mass, pos)]
+    turn(*[t.clone() for t in copies])                        # kernels loaded
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        turn(c.k, c.v, c.lengths, mass, pos)
+    for _ in range(3):
+        turn(*copies)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert c.lengths.tolist() == [100, 100, 100]
+    for a, b in zip((c.k, c.v, c.lengths, mass, pos), copies):
+        assert torch.equal(a.view(torch.int16) if a.dtype == torch.bfloat16 else a, b.view(torch.int16) if b.dtype == torch.bfloat16 else b)
 
 
 def test_evict_with_bad_pages_and_lengths():
