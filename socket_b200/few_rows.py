@@ -130,13 +130,17 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     """How likely `tokens` (int64, one per row, or None) were under logits [rows, vocab] (any number of rows), with the entropy
     of every row and its `top` (at most 64) likeliest tokens, the lower index first of equal ones.  fp32; logits are read once.  A
     row of nothing but -inf, or with NaN or +inf, gives NaN; so does a token outside the vocabulary, which also flags `status`."""
-    _require_cuda(logits)
-    dev = logits.device
-    _require_on(dev, tokens, status)
-    rows, vocab = logits.shape
+    index, dev = logits.get_device(), logits.device
+    if index < 0:
+        _require_cuda(logits)
+    if tokens is not None and tokens.get_device() != index or status is not None and status.get_device() != index:
+        _require_on(dev, tokens, status)
+    (rows, vocab), (ld, inner) = logits.shape, logits.stride()
     if not 0 <= top <= min(TOP_TOKENS, vocab):
         raise RuntimeError(f"token_logprobs: {top} alternatives of {vocab} tokens (at most {TOP_TOKENS})")
-    logits = _separate_rows(logits)                               # lives until the launch
+    if inner != 1 or ld < vocab:
+        logits = _separate_rows(logits)                           # lives until the launch
+        ld = _ld(logits)
     logprobs, f32 = None, torch.float32
     if tokens is not None:
         assert tokens.dtype == torch.int64 and tokens.numel() == rows
@@ -145,8 +149,8 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     found = TokenLogprobs(logprobs, torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, top, dtype=f32, device=dev),
                           torch.empty(rows, top, dtype=torch.int64, device=dev))
     step = library == "step"
-    on_device(dev.index, check if step else check_blocks, lib().sk_token_logprobs if step else blocks().skb_token_logprobs, "token_logprobs",
-              logits.data_ptr(), dtype_code(logits), _ld(logits), rows, vocab, ptr(tokens), top, ptr(logprobs), found[1].data_ptr(),
+    on_device(index, check if step else check_blocks, lib().sk_token_logprobs if step else blocks().skb_token_logprobs, "token_logprobs",
+              logits.data_ptr(), dtype_code(logits), ld, rows, vocab, ptr(tokens), top, ptr(logprobs), found[1].data_ptr(),
               found[2].data_ptr(), found[3].data_ptr(), ptr(status))
     return found
 

@@ -19,17 +19,28 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
-from ._lib import check, dtype_code, lib, on_device, ptr
+from ._lib import _raw_stream, check, dtype_code, lib, on_device, ptr
 
 # `sk_paged_cache` as bytes: filling in a ctypes structure field by field costs a call of a few microseconds another three
 _pack = struct.Struct("7P12q6i").pack
 
 
-def _same_device(index: int, *tensors: Optional[Tensor]) -> None:
+def _elsewhere(index: int, t: Tensor) -> RuntimeError:
     """Every tensor of a call lies on the device of its pools: the kernels read and write addresses."""
+    return RuntimeError(f"tensors of one call on device {index} and on {t.device}")
+
+
+def _same_device(index: int, *tensors: Optional[Tensor]) -> None:
     for t in tensors:
         if t is not None and t.get_device() != index:
-            raise RuntimeError(f"tensors of one call on device {index} and on {t.device}")
+            raise _elsewhere(index, t)
+
+
+def _run(index: int, entry, what: str, *args) -> None:
+    """entry(*args, stream) on the current stream of device `index`, the current device."""
+    status = entry(*args, torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index))
+    if status != 0:
+        check(status, what)
 
 
 def _cache(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass: Optional[Tensor], positions: Optional[Tensor],
@@ -38,7 +49,8 @@ def _cache(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mas
     index = k_pages.get_device()
     if index < 0:
         raise RuntimeError("socket_b200 operators need CUDA tensors (there is no CPU path)")
-    _same_device(index, v_pages, table, lengths, mass, positions, status)
+    if not index == v_pages.get_device() == table.get_device() == lengths.get_device():
+        _same_device(index, v_pages, table, lengths)
     shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
     n, G, page, D = shape
     B, width = table.shape
@@ -48,12 +60,18 @@ def _cache(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mas
     assert lengths.shape == (B,) and lengths.is_contiguous()
     mb = mh = pb = ph = 0
     if mass is not None:
+        if mass.get_device() != index:
+            raise _elsewhere(index, mass)
         assert mass.dtype == torch.float32
         mb, mh = _book(mass, B, G, width * page)
     if positions is not None:
+        if positions.get_device() != index:
+            raise _elsewhere(index, positions)
         assert positions.dtype == torch.int32
         pb, ph = _book(positions, B, G, width * page)
     if status is not None:
+        if status.get_device() != index:
+            raise _elsewhere(index, status)
         assert status.dtype == torch.int32 and status.numel() == 1
     return _pack(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), ptr(mass), ptr(positions), ptr(status),
                  ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], n, mb, mh, pb, ph, dtype_code(k_pages), B, G, D, page, width)
@@ -111,7 +129,7 @@ def attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Te
     B, H, D = shape
     assert B == table.shape[0] and D == k_pages.shape[3] and H % k_pages.shape[1] == 0 and q.dtype == k_pages.dtype and qs[2] == 1
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     os = out.stride()
     assert out.shape == shape and out.dtype == q.dtype and os[2] == 1
     entry = lib()
@@ -119,7 +137,7 @@ def attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Te
     have = 0 if workspace is None else workspace.numel() * workspace.element_size()
     if have < need:
         workspace, have = torch.empty(need, dtype=torch.uint8, device=q.device), need
-    on_device(index, check, entry.sk_paged_attn, "sk_paged_attn", c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], H, extra,
+    _run(index, entry.sk_paged_attn, "sk_paged_attn", c, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], H, extra,
               D ** -0.5 if scale is None else float(scale), ptr(workspace), have)
     return out
 
@@ -139,8 +157,8 @@ def evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass
             return evict(k_pages, v_pages, table, lengths, mass, positions, budget=budget, recent=recent, sink=sink, out=out, status=status)
     B, G, slots = table.shape[0], k_pages.shape[1], table.shape[1] * k_pages.shape[2]
     if out is None:
-        out = (torch.empty(B, G, slots, dtype=torch.float32, device=dev), torch.empty(B, G, slots, dtype=torch.int32, device=dev),
-               torch.empty(B, dtype=torch.int32, device=dev))
+        out = tuple(torch.empty_like(t if t.shape[2] == slots else t[..., :slots], memory_format=torch.contiguous_format)
+                    for t in (mass, positions)) + (torch.empty_like(lengths),)
     m, q, n = out
     _same_device(index, m, q, n)
     assert m.dtype == torch.float32 and q.dtype == n.dtype == torch.int32 and n.shape == lengths.shape and n.is_contiguous()
@@ -148,7 +166,7 @@ def evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass
     entry = lib()
     need = entry.sk_paged_evict_workspace_bytes(c, budget)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    on_device(index, check, entry.sk_paged_evict, "sk_paged_evict", c, budget, recent, sink, m.data_ptr(), mb, mh, q.data_ptr(), pb, ph,
+    _run(index, entry.sk_paged_evict, "sk_paged_evict", c, budget, recent, sink, m.data_ptr(), mb, mh, q.data_ptr(), pb, ph,
               n.data_ptr(), ptr(ws), need)
     return out
 
