@@ -97,6 +97,9 @@ template <> __device__ __forceinline__ float pt_high<__half>(uint32_t x) { retur
 __device__ __forceinline__ float pt_factor(float a, float b) { return exp2_fast(a - (b == -INFINITY ? 0.f : b)); }
 __device__ __forceinline__ float pt_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// 64-bit division is some hundred instructions in a row, and chunks are rarely that many
+__device__ __forceinline__ int64_t pt_div(int64_t a, int64_t b) { return (uint64_t)(a | b) >> 32 == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
+
 // A place in the row of chunks: chunk `chunk` of `chunks` of group grp of key/value head g of sequence b, which has n keys.  Behind the
 // chunks of every group stand PT_PAD empty ones: what it costs a block to finish it and begin the next.
 constexpr int PT_PAD = 1;
@@ -163,7 +166,7 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
     for (int b = blockIdx.x; b < c.B; b += gridDim.x)          // no key, no run: zeros
         if (paged_length(c, b, a.extra) == 0)
             for (int i = t; i < a.H * c.D; i += S::THREADS) ((T*)a.out)[b * a.o_bs + i / c.D * a.o_hs + i % c.D] = from_f32<T>(0.f);
-    const int64_t per = (total + gridDim.x - 1) / gridDim.x, first = per * blockIdx.x;
+    const int64_t per = pt_div(total + gridDim.x - 1, gridDim.x), first = per * blockIdx.x;
     int left = (int)max(min(per, total - first), (int64_t)0);
     PtRun* run = a.runs == nullptr ? nullptr : a.runs + blockIdx.x;
     if (run != nullptr && t == 0) {
@@ -172,8 +175,8 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
     }
     if (left == 0) return;
     auto place = [&](int b, int n, int64_t lo) {               // of chunk `first` in sequence b, whose chunks begin at lo
-        const int m = slots_of(n), unit = (int)((first - lo) / m);
-        return PtPlace{b, unit / a.groups, unit % a.groups, (int)((first - lo) % m), m - PT_PAD, n};
+        const int m = slots_of(n), unit = (int)pt_div(first - lo, m);
+        return PtPlace{b, unit / a.groups, unit % a.groups, (int)(first - lo - (int64_t)unit * m), m - PT_PAD, n};
     };
     if (few) {
         const int b = __ffs(__ballot_sync(FULL, before * units > first)) - 1, n = __shfl_sync(FULL, n_lane, b);
@@ -576,7 +579,7 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
         run->tail_g = cur.g;
         run->tail_grp = cur.grp;
         run->tail_inside = !seg_first;
-        run->tail_last = (int)((flat - cur.chunk + cur.chunks - 1) / per);
+        run->tail_last = (int)pt_div(flat - cur.chunk + cur.chunks - 1, per);
     }
 }
 
@@ -668,47 +671,53 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
             for (int grp = 0; grp < a.groups; ++grp) {
                 const int heads = min(HG, rep - grp * HG);
                 const int64_t begin = flat - p.chunk + (int64_t)grp * (p.chunks + PT_PAD);
-                const int y0 = (int)(begin / per), y1 = (int)((begin + p.chunks - 1) / per);
+                const int y0 = (int)pt_div(begin, per), y1 = (int)pt_div(begin + p.chunks - 1, per);
+                const float* sc = a.scores + begin * CHUNK * a.rs;
+                // four heads a key: the first keys' scores and masses are asked for before the heads' maxima are
+                float4 x[4];
+                float w[4];
+                auto ask = [&](int j) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (j + u * 32 < j1) {
+                            x[u] = __ldcs(reinterpret_cast<const float4*>(sc) + j + u * 32);
+                            w[u] = mass[j + u * 32];
+                        }
+                };
+                if (a.rs == 4) ask(j0 + lane);
                 __syncwarp();
-                if (y0 == y1 && lane < heads) {                // final maximum and 1 / sum: there already
-                    const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)p.b * a.H + g * rep + grp * HG + lane) * 2));
-                    stat[0][lane] = st.x == -INFINITY ? 0.f : st.x;
-                    stat[1][lane] = st.y;
-                }
-                if (y0 != y1)
-                    for (int h = 0; h < heads; ++h) {
-                        float m = -INFINITY, l = 0.f;
-                        for (int x = y0 + lane; x <= y1; x += 32) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pt_part<S>(a, x, begin > x * per) + HG * DP + h * 2));
+                if (y0 == y1) {                                // final maximum and 1 / sum: there already
+                    if (lane < heads) {
+                        const float2 st = __ldcg(reinterpret_cast<const float2*>(a.stats + ((int64_t)p.b * a.H + g * rep + grp * HG + lane) * 2));
+                        stat[0][lane] = st.x == -INFINITY ? 0.f : st.x;
+                        stat[1][lane] = st.y;
+                    }
+                } else {                                       // as many lanes for every head
+                    const int of_head = heads <= 4 ? 8 : heads <= 8 ? 4 : 2, h = lane / of_head;
+                    float m = -INFINITY, l = 0.f;
+                    if (h < heads)
+                        for (int y = y0 + lane % of_head; y <= y1; y += of_head) {
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pt_part<S>(a, y, begin > y * per) + HG * DP + h * 2));
                             const float mn = fmaxf(m, ml.x);
                             l = l * pt_factor(m, mn) + ml.y * pt_factor(ml.x, mn);
                             m = mn;
                         }
-#pragma unroll
-                        for (int o = 16; o >= 1; o >>= 1) {
-                            const float m2 = __shfl_xor_sync(FULL, m, o), l2 = __shfl_xor_sync(FULL, l, o), mn = fmaxf(m, m2);
-                            l = l * pt_factor(m, mn) + l2 * pt_factor(m2, mn);
-                            m = mn;
-                        }
-                        if (lane == 0) {
-                            stat[0][h] = m == -INFINITY ? 0.f : m;
-                            stat[1][h] = pt_inverse(l);
-                        }
+                    for (int o = of_head / 2; o >= 1; o >>= 1) {
+                        const float m2 = __shfl_xor_sync(FULL, m, o), l2 = __shfl_xor_sync(FULL, l, o), mn = fmaxf(m, m2);
+                        l = l * pt_factor(m, mn) + l2 * pt_factor(m2, mn);
+                        m = mn;
                     }
+                    if (h < heads && lane % of_head == 0) {
+                        stat[0][h] = m == -INFINITY ? 0.f : m;
+                        stat[1][h] = pt_inverse(l);
+                    }
+                }
                 __syncwarp();
-                const float* sc = a.scores + begin * CHUNK * a.rs;
                 if (a.rs == 4) {
                     const float4 m4 = make_float4(stat[0][0], stat[0][1], stat[0][2], stat[0][3]);
-                    const float4 l4 = make_float4(stat[1][0], stat[1][1], stat[1][2], heads > 3 ? stat[1][3] : 0.f);
+                    const float4 l4 = make_float4(stat[1][0], stat[1][1], stat[1][2], stat[1][3]);
                     for (int j = j0 + lane; j < j1; j += 128) {
-                        float4 x[4];
-                        float w[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (j + u * 32 < j1) {
-                                x[u] = __ldcs(reinterpret_cast<const float4*>(sc) + j + u * 32);
-                                w[u] = mass[j + u * 32];
-                            }
+                        if (j >= j0 + 128) ask(j);
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             if (j + u * 32 < j1) {
@@ -720,11 +729,26 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                             }
                     }
                 } else {
+                    const int vec = a.rs % 4 == 0 ? 4 : 2;
 #pragma unroll 2
                     for (int j = j0 + lane; j < j1; j += 32) {
-                        float w = 0.f;
-                        for (int h = 0; h < heads; ++h) w = fmaf(exp2_fast(__ldcg(sc + (int64_t)j * a.rs + h) - stat[0][h]), stat[1][h], w);
-                        mass[j] += w;
+                        const float* row = sc + (int64_t)j * a.rs;
+                        const float old = mass[j];
+                        float s = 0.f;
+                        for (int h = 0; h < heads; h += vec) {
+                            float4 v;
+                            if (vec == 4) {
+                                v = __ldcs(reinterpret_cast<const float4*>(row + h));
+                            } else {
+                                const float2 two = __ldcs(reinterpret_cast<const float2*>(row + h));
+                                v = make_float4(two.x, two.y, 0.f, 0.f);
+                            }
+                            s = fmaf(exp2_fast(v.x - stat[0][h]), stat[1][h], s);
+                            if (h + 1 < heads) s = fmaf(exp2_fast(v.y - stat[0][h + 1]), stat[1][h + 1], s);
+                            if (vec == 4 && h + 2 < heads) s = fmaf(exp2_fast(v.z - stat[0][h + 2]), stat[1][h + 2], s);
+                            if (vec == 4 && h + 3 < heads) s = fmaf(exp2_fast(v.w - stat[0][h + 3]), stat[1][h + 3], s);
+                        }
+                        mass[j] = old + s;
                     }
                 }
             }
