@@ -11,9 +11,9 @@
 // pair, or ends, the block's warps join; a pair inside one run is then finished, others leave a partial result for a second kernel.
 // The second kernel also adds the weights to mass, from scores that the first one leaves behind (they need the final maximum and sum).
 //
-// Measured, 32 / 8 heads of 128: 32768 keys 30 us (134 MB; first kernel 26 at 5.1 TB/s, the start and end of a block's run 5 of them), 4 x 131072 with
-// mass 380 us (350 at 6.3 TB/s and 25), 64 sequences of 1 to 8003 with mass 61 us (49 and 11).  Eight warps a block and one block an SM: with
-// two blocks of four the ragged batch takes 62.6, the long one 383.  A pair's end counted as one chunk: as two 63, measured in tiles of 16 62 to 113.
+// Measured, 32 / 8 heads of 128: 32768 keys 29 us (134 MB; first kernel 26 at 5.1 TB/s, the start and end of a block's run 5 of them), 4 x 131072 with
+// mass 376 us (350 at 6.3 TB/s and 25), 64 sequences of 1 to 8003 with mass 57.5 us (49 and 8).  Eight warps a block and one block an SM: two blocks of
+// four cost the ragged batch 2 us and the long one 4.  A pair's end counted as one chunk: as two 3 us more, with work measured in tiles 1 to 50.
 //
 // 16-bit types: S^T = K Q^T and O^T = V^T P^T by m16n8k16 products, keys and then value columns in the 16 rows and up to 8 query heads in
 // the 8 columns, which wastes half of what heads in the rows would.  Weights go in as two halves (value and rounding rest), so that what is

@@ -1,13 +1,13 @@
 // Eviction from a paged cache by collected attention weight.
 //
-// First kernel, a cluster per (sequence, key/value head): slots are ranked by a 32-bit key that grows with their mass; the key of the
+// A cluster per (sequence, key/value head): slots are ranked by a 32-bit key that grows with their mass; the key of the
 // last slot to be kept is found by four histograms of eight bits, summed over the cluster, and equal keys go by slot.  Then every slot
-// is kept or not, and the i-th freed slot below the budget and the i-th kept one behind it are written side by side.  Second kernel: a
-// list entry is a row of K, a row of V, a mass and a position to move; sources lie behind the budget and targets below it, so
-// entries may go in any order.  Only what moves is read: mass and positions once, 241 of 4352 keys of D elements.
+// is kept or not, and the i-th freed slot below the budget and the i-th kept one behind it are written side by side.  A
+// list entry is a row of K, a row of V, a mass and a position to move; sources lie behind the budget and targets below it, so the
+// cluster's blocks move entries in any order once the list is complete.  Only what moves is read: mass and positions once, 241 of 4352 keys of D elements.
 //
-// Measured, 8 heads of 128: 32 sequences from 4352 to 4096 slots 31 us (18 + 13: the first kernel waits in four passes of three barriers each, the
-// second moves 63 MB), one from 32768 to 4096 28 us (17 + 11; its passes end in barriers of the cluster).
+// Measured, 8 heads of 128: 32 sequences from 4352 to 4096 slots 28 us (about 17 in four passes of three barriers each, then 63 MB of rows), one from
+// 32768 to 4096 29 us (its passes end in barriers of the cluster).  With the moves in a kernel of their own 31 and 28, and a launch more.
 #include "paged.cuh"
 
 #include <type_traits>
@@ -16,16 +16,15 @@ namespace sk {
 namespace {
 
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 8;
+// Moves a thread has under way: many rows share an SM by two blocks, a cluster's are few
+template <int CL> constexpr int EV_MOVES_OF = CL == 1 ? 2 : 4;
+template <int CL> constexpr int EV_PER_SM = CL == 1 ? 2 : 1;
 constexpr int EV_SLOTS = 24576;                                // of a block, whose keys and positions find room in shared memory
 struct alignas(16) EvMove {
     int from, to;
     float mass;
     int pos;
 };
-struct EvRow {
-    int moves, length;
-};
-
 struct EvShared {
     uint32_t hist[2][256], total[256];
     int newest, equals, holes, movers;                         // of this block; read by the cluster
@@ -52,9 +51,9 @@ template <int CL> __device__ __forceinline__ void ev_sync() {
 }
 
 template <int CL>
-__global__ void __launch_bounds__(EV_THREADS)
+__global__ void __launch_bounds__(EV_THREADS, EV_PER_SM<CL>)
 paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs,
-                   int32_t* pos_out, int64_t po_bs, int64_t po_hs, EvRow* rows, EvMove* moves, int most_moves, int room) {
+                   int32_t* pos_out, int64_t po_bs, int64_t po_hs, int32_t* lengths_out, EvMove* moves, int most_moves, int room) {
     pdl_begin();
     extern __shared__ uint32_t ev_raw[];                       // keys, then positions of this block's slots
     __shared__ EvShared s;
@@ -68,7 +67,7 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
     const int n = paged_length(c, b, 0, &over), kept = min(n, budget);
     if (rank == 0 && t == 0) {
         if (over && c.status != nullptr) atomicOr(c.status, SK_DEV_POS_OUT_OF_RANGE);
-        if (n <= budget) rows[row] = EvRow{0, kept};
+        if (lengths_out != nullptr && g == 0) lengths_out[b] = kept;
     }
     for (int j = n + rank * EV_THREADS + t; j < cap; j += CL * EV_THREADS) {
         mo[j] = 0.f;
@@ -87,6 +86,8 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
     if (t == 0) s.newest = INT32_MIN;
     for (int i = t; i < 256; i += EV_THREADS) s.hist[0][i] = 0;
     __syncthreads();
+    EvMove* list = moves + (int64_t)row * most_moves;
+    int moves_n = 0;
     auto select = [&](auto on_chip) {
         constexpr bool HELD = decltype(on_chip)::value;        // keys and positions in shared memory; else they are read again
         uint32_t* keys = ev_raw;
@@ -230,8 +231,7 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
             }
             all_movers = sum;
         }
-        if (rank == 0 && t == 0) rows[row] = EvRow{all_movers, kept};
-        EvMove* list = moves + (int64_t)row * most_moves;
+        moves_n = all_movers;
         seen = equal_at;
         constexpr int STEPS = 4;                               // whose masses are asked for at a time
         for (int first = i0; first < i1; first += 32 * STEPS) {
@@ -266,63 +266,63 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
     };
     if (share <= room) select(std::true_type{});
     else select(std::false_type{});
-    if (CL > 1) ev_sync<CL>();                                 // no block leaves while others read its counts
+    ev_sync<CL>();                                             // the list is complete, and the others' counts are read
+
+    // ---- moves: a thread per 16-byte piece of some of them
+    constexpr int EV_MOVES = EV_MOVES_OF<CL>;
+    const int es = c.dtype == SK_F32 ? 4 : 2, pieces = c.D * es / 16, per = 1 << (32 - __clz(pieces - 1)), p = t & (per - 1);
+    const int step = EV_THREADS / per, shift = 31 - __clz(c.page);
+    for (int i0 = rank * EV_MOVES * step + t / per; i0 < moves_n; i0 += CL * EV_MOVES * step) {
+        int4 e[EV_MOVES];
+        int from[EV_MOVES], to[EV_MOVES];
+#pragma unroll
+        for (int x = 0; x < EV_MOVES; ++x)
+            if (i0 + x * step < moves_n) e[x] = __ldcg(reinterpret_cast<const int4*>(list + i0 + x * step));
+#pragma unroll
+        for (int x = 0; x < EV_MOVES; ++x)
+            if (i0 + x * step < moves_n) {
+                from[x] = __ldcg(c.table + b * c.table_ld + (e[x].x >> shift));
+                to[x] = __ldcg(c.table + b * c.table_ld + (e[x].y >> shift));
+            }
+        uint4 k[EV_MOVES], v[EV_MOVES];
+        bool ok[EV_MOVES];
+#pragma unroll
+        for (int x = 0; x < EV_MOVES; ++x) {
+            ok[x] = i0 + x * step < moves_n && paged_page_ok(c, from[x]) && paged_page_ok(c, to[x]);
+            if (ok[x] && p < pieces) {
+                const int r = e[x].x & (c.page - 1);
+                k[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.k + (from[x] * c.k_ps + g * c.k_hs + r * c.k_rs) * es) + p);
+                v[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.v + (from[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es) + p);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < EV_MOVES; ++x) {
+            if (i0 + x * step >= moves_n) continue;
+            if (ok[x] && p < pieces) {
+                const int r = e[x].y & (c.page - 1);
+                reinterpret_cast<uint4*>((char*)c.k + (to[x] * c.k_ps + g * c.k_hs + r * c.k_rs) * es)[p] = k[x];
+                reinterpret_cast<uint4*>((char*)c.v + (to[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es)[p] = v[x];
+            }
+            if (p == 0) {
+                mo[e[x].y] = __int_as_float(e[x].z);
+                po[e[x].y] = e[x].w;
+                if (!ok[x] && c.status != nullptr) atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
+            }
+        }
+    }
 }
 
-// A thread per 16-byte piece of four moves of its own
-constexpr int EM_THREADS = 256, EM_MOVES = 4;
-__global__ void __launch_bounds__(EM_THREADS)
-paged_move_kernel(const __grid_constant__ sk_paged_cache c, float* mass_out, int64_t mo_bs, int64_t mo_hs, int32_t* pos_out, int64_t po_bs, int64_t po_hs,
-                  int32_t* lengths_out, const EvRow* rows, const EvMove* moves, int most_moves, int es, int pieces, int blocks) {
+// New lengths in place of the old ones, which blocks of the kernel before read
+__global__ void __launch_bounds__(256)
+paged_evict_lengths_kernel(const __grid_constant__ sk_paged_cache c, int budget, int32_t* lengths_out) {
     pdl_begin();
-    const int row = blockIdx.x / blocks, part = blockIdx.x % blocks, g = row % c.G, b = row / c.G;
-    const int n = __ldcg(&rows[row].moves);
-    if (part == 0 && g == 0 && threadIdx.x == 0) lengths_out[b] = __ldcg(&rows[row].length);
-    const int per = 1 << (32 - __clz(pieces - 1)), p = threadIdx.x & (per - 1), step = EM_THREADS / per, shift = 31 - __clz(c.page);
-    const int i0 = part * EM_MOVES * step + threadIdx.x / per;
-    if (part * EM_MOVES * step >= n) return;
-    const EvMove* list = moves + (int64_t)row * most_moves;
-    int4 e[EM_MOVES];
-    int from[EM_MOVES], to[EM_MOVES];
-#pragma unroll
-    for (int x = 0; x < EM_MOVES; ++x)
-        if (i0 + x * step < n) e[x] = __ldcg(reinterpret_cast<const int4*>(list + i0 + x * step));
-#pragma unroll
-    for (int x = 0; x < EM_MOVES; ++x)
-        if (i0 + x * step < n) {
-            from[x] = __ldcg(c.table + b * c.table_ld + (e[x].x >> shift));
-            to[x] = __ldcg(c.table + b * c.table_ld + (e[x].y >> shift));
-        }
-    uint4 k[EM_MOVES], v[EM_MOVES];
-    bool ok[EM_MOVES];
-#pragma unroll
-    for (int x = 0; x < EM_MOVES; ++x) {
-        ok[x] = i0 + x * step < n && paged_page_ok(c, from[x]) && paged_page_ok(c, to[x]);
-        if (ok[x] && p < pieces) {
-            const int r = e[x].x & (c.page - 1);
-            k[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.k + (from[x] * c.k_ps + g * c.k_hs + r * c.k_rs) * es) + p);
-            v[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.v + (from[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es) + p);
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < EM_MOVES; ++x) {
-        if (i0 + x * step >= n) continue;
-        if (ok[x] && p < pieces) {
-            const int r = e[x].y & (c.page - 1);
-            reinterpret_cast<uint4*>((char*)c.k + (to[x] * c.k_ps + g * c.k_hs + r * c.k_rs) * es)[p] = k[x];
-            reinterpret_cast<uint4*>((char*)c.v + (to[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es)[p] = v[x];
-        }
-        if (p == 0) {
-            mass_out[b * mo_bs + g * mo_hs + e[x].y] = __int_as_float(e[x].z);
-            pos_out[b * po_bs + g * po_hs + e[x].y] = e[x].w;
-            if (!ok[x] && c.status != nullptr) atomicOr(c.status, SK_DEV_INDEX_OUT_OF_RANGE);
-        }
-    }
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b < c.B) lengths_out[b] = min(paged_length(c, b, 0), budget);
 }
 
 struct EvPlan {
     int cluster, room, most_moves;
-    size_t moves, total;                                       // bytes in front of the lists, and of all
+    size_t total;                                              // bytes of the lists
 };
 EvPlan ev_plan(const sk_paged_cache& c, int budget) {
     EvPlan p;
@@ -336,14 +336,13 @@ EvPlan ev_plan(const sk_paged_cache& c, int budget) {
     p.room = (int)(share < EV_SLOTS ? share : EV_SLOTS);
     const int64_t behind = cap > budget ? cap - budget : 0;
     p.most_moves = (int)(behind < budget ? behind : budget);
-    p.moves = up256((size_t)rows * sizeof(EvRow));
-    p.total = p.moves + (size_t)rows * p.most_moves * sizeof(EvMove);
+    p.total = (size_t)rows * p.most_moves * sizeof(EvMove);
     return p;
 }
 
 template <int CL>
 int evict_launch(const sk_paged_cache& c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs, int32_t* pos_out,
-                 int64_t po_bs, int64_t po_hs, EvRow* rows, EvMove* moves, const EvPlan& p, cudaStream_t st) {
+                 int64_t po_bs, int64_t po_hs, int32_t* lengths_out, EvMove* moves, const EvPlan& p, cudaStream_t st) {
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)paged_evict_kernel<CL>, (size_t)EV_SLOTS * 8);
     if (e != cudaSuccess) return check_chained(e, "paged_evict_kernel");
@@ -360,7 +359,7 @@ int evict_launch(const sk_paged_cache& c, int budget, int recent, int sink, floa
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = CL > 1 ? 2 : 1;
-    return check_chained(cudaLaunchKernelEx(&cfg, paged_evict_kernel<CL>, c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, rows,
+    return check_chained(cudaLaunchKernelEx(&cfg, paged_evict_kernel<CL>, c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, lengths_out,
                                             moves, p.most_moves, p.room), "paged_evict_kernel");
 }
 
@@ -371,20 +370,14 @@ size_t paged_evict_workspace(const sk_paged_cache& c, int budget) { return ev_pl
 int launch_paged_evict(const sk_paged_cache& c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs,
                        int32_t* pos_out, int64_t po_bs, int64_t po_hs, int32_t* lengths_out, void* workspace, cudaStream_t st) {
     const EvPlan p = ev_plan(c, budget);
-    EvRow* rows = (EvRow*)workspace;
-    EvMove* moves = (EvMove*)((char*)workspace + p.moves);
-    const int es = (int)esize(c.dtype), pieces = c.D * es / 16;
-    int per = 1;
-    while (per < pieces) per *= 2;
-    const int of_block = EM_MOVES * (EM_THREADS / per);
-    const int blocks = p.most_moves > 0 ? (p.most_moves + of_block - 1) / of_block : 1;
-    if ((int64_t)c.B * c.G * blocks > INT32_MAX || (int64_t)c.B * c.G * EV_CLUSTER > INT32_MAX)
-        return fail(SK_ERR_UNSUPPORTED, "sk_paged_evict: %d sequences with %d heads and a budget of %d", c.B, c.G, budget);
+    if ((int64_t)c.B * c.G * EV_CLUSTER > INT32_MAX) return fail(SK_ERR_UNSUPPORTED, "sk_paged_evict: %d sequences with %d heads", c.B, c.G);
+    const bool apart = lengths_out + c.B <= c.lengths || c.lengths + c.B <= lengths_out;
     auto go = p.cluster == 8 ? evict_launch<8> : p.cluster == 4 ? evict_launch<4> : p.cluster == 2 ? evict_launch<2> : evict_launch<1>;
-    if (int rc = go(c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, rows, moves, p, st)) return rc;
-    return check_chained(launch_after(paged_move_kernel, dim3((unsigned)(c.B * c.G * blocks)), dim3(EM_THREADS), 0, st, c, mass_out, mo_bs, mo_hs, pos_out,
-                                      po_bs, po_hs, lengths_out, (const EvRow*)rows, (const EvMove*)moves, p.most_moves, es, pieces, blocks),
-                         "paged_move_kernel");
+    if (int rc = go(c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, apart ? lengths_out : nullptr, (EvMove*)workspace, p, st))
+        return rc;
+    if (apart) return SK_OK;
+    return check_chained(launch_after(paged_evict_lengths_kernel, dim3((unsigned)((c.B + 255) / 256)), dim3(256), 0, st, c, budget, lengths_out),
+                         "paged_evict_lengths_kernel");
 }
 
 }  // namespace sk
