@@ -7,7 +7,8 @@
 // cluster's blocks move entries in any order once the list is complete.  Only what moves is read: mass and positions once, 241 of 4352 keys of D elements.
 //
 // Measured, 8 heads of 128: 32 sequences from 4352 to 4096 slots 28 us (about 17 in four passes of three barriers each, then 63 MB of rows), one from
-// 32768 to 4096 29 us (its passes end in barriers of the cluster).  With the moves in a kernel of their own 31 and 28, and a launch more.
+// 32768 to 4096 27.7 us (15 until its moves begin: passes end in barriers of the cluster).  With the moves in a kernel of their own 31 and 28, and a
+// launch more; with three histograms of 2048 bins 29 and 52, words of other blocks cost that much.
 #include "paged.cuh"
 
 #include <type_traits>
@@ -35,12 +36,23 @@ struct EvShared {
 // What a slot is ranked by: slots kept for sure above all, NaN above numbers
 __device__ __forceinline__ uint32_t ev_key(float mass) { return mass != mass ? 0xFFFFFFFEu : min(order_key(mass), 0xFFFFFFFEu); }
 
-// a word of another block's shared memory, at the place `local` has in this one's
-__device__ __forceinline__ uint32_t ev_remote(const void* local, int rank) {
-    uint32_t at, v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
+// A word of every block's shared memory, at the place `local` has in this one's, all asked for before the first is used; the caller has
+// passed a cluster barrier behind their writes
+template <int CL> __device__ __forceinline__ void ev_remote(const void* local, uint32_t (&v)[CL]) {
+    uint32_t at[CL];
+#pragma unroll
+    for (int r = 0; r < CL; ++r) asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at[r]) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(r));
+    if constexpr (CL == 8) {
+        asm volatile(
+            "ld.shared::cluster.u32 %0, [%8];\n\tld.shared::cluster.u32 %1, [%9];\n\tld.shared::cluster.u32 %2, [%10];\n\t"
+            "ld.shared::cluster.u32 %3, [%11];\n\tld.shared::cluster.u32 %4, [%12];\n\tld.shared::cluster.u32 %5, [%13];\n\t"
+            "ld.shared::cluster.u32 %6, [%14];\n\tld.shared::cluster.u32 %7, [%15];"
+            : "=&r"(v[0]), "=&r"(v[1]), "=&r"(v[2]), "=&r"(v[3]), "=&r"(v[4]), "=&r"(v[5]), "=&r"(v[6]), "=&r"(v[7])
+            : "r"(at[0]), "r"(at[1]), "r"(at[2]), "r"(at[3]), "r"(at[4]), "r"(at[5]), "r"(at[6]), "r"(at[7]) : "memory");
+    } else {
+#pragma unroll
+        for (int r = 0; r < CL; ++r) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[r]) : "r"(at[r]) : "memory");
+    }
 }
 template <int CL> __device__ __forceinline__ void ev_sync() {
     if (CL == 1) __syncthreads();
@@ -106,8 +118,12 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         if (lane == 0) atomicMax(&s.newest, newest);
         ev_sync<CL>();
         newest = s.newest;
-        if (CL > 1)
-            for (int k = 0; k < CL; ++k) newest = max(newest, (int)ev_remote(&s.newest, k));
+        if constexpr (CL > 1) {
+            uint32_t v[CL];
+            ev_remote<CL>(&s.newest, v);
+#pragma unroll
+            for (int r = 0; r < CL; ++r) newest = max(newest, (int)v[r]);
+        }
         const int late = (int)max((int64_t)newest - recent, (int64_t)INT32_MIN);
         auto sure = [&](int p) { return p < sink || p > late; };
         auto key = [&](int i) {                                // of slot j0 + i, after the first pass
@@ -140,10 +156,12 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
             ev_sync<CL>();
             if (t < 256) {
                 uint32_t sum = hist[t];
-                if (CL > 1) {
+                if constexpr (CL > 1) {
+                    uint32_t v[CL];
+                    ev_remote<CL>(hist + t, v);
                     sum = 0;
 #pragma unroll
-                    for (int x = 0; x < CL; ++x) sum += ev_remote(hist + t, x);
+                    for (int r = 0; r < CL; ++r) sum += v[r];
                 }
                 s.total[t] = sum;
                 s.hist[(pass + 1) & 1][t] = 0;                 // read by the others before the barrier
@@ -188,10 +206,13 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
             int equal = 0;
             for (int i = i0 + lane; i - lane < i1; i += 32) equal += __popc(__ballot_sync(FULL, i < i1 && key(i) == prefix));
             equal_at = before(0, equal, all);
-            if (CL > 1) {
+            if constexpr (CL > 1) {
                 if (t == 0) s.equals = all;
                 ev_sync<CL>();
-                for (int x = 0; x < rank; ++x) equal_at += (int)ev_remote(&s.equals, x);
+                uint32_t v[CL];
+                ev_remote<CL>(&s.equals, v);
+#pragma unroll
+                for (int r = 0; r < CL; ++r) equal_at += r < rank ? (int)v[r] : 0;
             }
         }
         // one step of the walk over a warp's run: is slot i kept
@@ -213,23 +234,22 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         holes = __reduce_add_sync(FULL, holes);
         movers = __reduce_add_sync(FULL, movers);
         int all_holes, all_movers, hole_at = before(1, holes, all_holes), mover_at = before(2, movers, all_movers);
-        if (CL > 1) {
+        if constexpr (CL > 1) {
             if (t == 0) {
                 s.holes = all_holes;
                 s.movers = all_movers;
             }
             ev_sync<CL>();
-            int sum = 0;
+            uint32_t h[CL], m[CL];
+            ev_remote<CL>(&s.holes, h);
+            ev_remote<CL>(&s.movers, m);
+            all_movers = 0;
 #pragma unroll
-            for (int x = 0; x < CL; ++x) {
-                const int h = (int)ev_remote(&s.holes, x), m = (int)ev_remote(&s.movers, x);
-                if (x < rank) {
-                    hole_at += h;
-                    mover_at += m;
-                }
-                sum += m;
+            for (int r = 0; r < CL; ++r) {
+                hole_at += r < rank ? (int)h[r] : 0;
+                mover_at += r < rank ? (int)m[r] : 0;
+                all_movers += (int)m[r];
             }
-            all_movers = sum;
         }
         moves_n = all_movers;
         seen = equal_at;
