@@ -231,9 +231,9 @@ def generate(model: Decoder, prompt: Tensor, max_new_tokens: int, mode: Optional
     [B, T + max_new_tokens], stats) with `decode_time_s` measured by CUDA events around the decode
     loop and `decode_only_tokens = B * (max_new_tokens - 1)` (generate.py:362-368).  `prompt` may be
     a host tensor; with `stream_to_host` every new token is copied to pinned host memory and waited
-    for before the next step is launched (the end-to-end serving pattern).  With `logprobs` (a number of alternatives, 0 for none)
-stats["logprobs"] tells how likely the new tokens were: log probabilities and entropies [B, max_new_tokens], and the likeliest
-tokens with theirs [B, max_new_tokens, logprobs]."""
+    for before the next step is launched (the end-to-end serving pattern).  With `logprobs` (a number of
+    alternatives, 0 for none) stats["logprobs"] tells how likely the new tokens were: log probabilities and
+    entropies [B, max_new_tokens], and the likeliest tokens with theirs [B, max_new_tokens, logprobs]."""
     dev = model.device
     B, T = prompt.shape
     prompt_d = prompt.to(dev, non_blocking=True)

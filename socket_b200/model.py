@@ -423,23 +423,26 @@ class Transformer(Decoder):
         if mode is not None and (mode == "paged") != (self.paging is not None):
             self.use_pages(Paging() if mode == "paged" else None)
 
+    def setup_caches(self, max_batch_size: int, max_seq_length: int) -> None:
+        if self.pages is not None and max_batch_size != self.pages.table.shape[0]:
+            self.max_batch_size = -1                    # sequences in pages grow in step: caches are for one number of them
+        super().setup_caches(max_batch_size, max_seq_length)
+
     def _alloc_caches(self, batch: int, length: int) -> None:
-        """Per-layer caches (K, V, bucket codes, value norms) and the rotary table; as
+        """Per-layer caches (K, V, bucket codes, value norms, or K and V in pages) and the rotary table; as
         GPT-FAST/model.py:251-278 minus the T x T mask."""
-        if self.paging is not None:
-            p = self.paging
-            self.pages = PageTable(batch, length, p.page, p.pages, self.device)
-        for b in self.layers if self.paging is not None else ():
-            a = b.attention
-            a.kv_cache = PagedKVCache(self.pages, a.n_local_heads, a.head_dim, dtype=self.dtype, device=self.device, collect=p.budget > 0)
-        self.freqs_cis = precompute_freqs_cis(min(self.config.block_size, length), self.config.head_dim,
-                                              self.config.rope_base, device=self.device)
-        if self.paging is not None:
-            return
+        paging = self.paging
+        if paging is not None:
+            self.pages = PageTable(batch, length, paging.page, paging.pages, self.device)
         for b in self.layers:
             a = b.attention
+            if paging is not None:
+                a.kv_cache = PagedKVCache(self.pages, a.n_local_heads, a.head_dim, dtype=self.dtype, device=self.device, collect=paging.budget > 0)
+                continue
             a.kv_cache = KVCache(batch, length, a.n_local_heads, a.head_dim, L=a.L, R=a.R, dtype=self.dtype,
                                  device=self.device)
+        self.freqs_cis = precompute_freqs_cis(min(self.config.block_size, length), self.config.head_dim,
+                                              self.config.rope_base, device=self.device)
 
     # ------------------------------------------------------------------------------- prefill
     def _portion(self, idx: Tensor, start: int) -> Tensor:

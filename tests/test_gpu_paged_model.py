@@ -129,6 +129,10 @@ def test_calls_that_pages_refuse():
     plain.setup_caches(2, 100)
     with pytest.raises(RuntimeError, match="pages"):
         plain.setup_decode(2, "paged", use_graph=False)
+    # other numbers of sequences get caches of their own
+    for B in (1, 3):
+        seq, _ = generate(model, _prompt(B, 30), 5)
+        assert seq.shape == (B, 35) and model.pages.lengths.tolist() == [34] * B
     # and back again
     generate(model, prompt.cpu(), 5, mode="sparse")
     assert model.pages is None
