@@ -156,9 +156,8 @@ constexpr int lp_room(int top, int of_thread) { return (top + LP_FEW) * of_threa
 template <int THREADS> __device__ __forceinline__ int lp_cut(LpShared<THREADS>& s, int n, int top) {
     const int t = threadIdx.x;
     if (n > LP_RANKED) {                                       // the top-th pair by halving, then what reaches it
-        LpPair lo = 0, hi = ~0ull;                             // at least `top` reach lo, fewer reach hi
-        while (hi - lo > 1) {
-            const LpPair mid = lo + (hi - lo) / 2;
+        LpPair lo = 0, hi = ~0ull, mid = hi;                   // at least `top` reach lo; fewer reach hi, once that is tested
+        for (;;) {
             __syncthreads();
             if (t == 0) s.count = 0;
             __syncthreads();
@@ -170,7 +169,8 @@ template <int THREADS> __device__ __forceinline__ int lp_cut(LpShared<THREADS>& 
             c = s.count;
             if (c >= top) lo = mid;
             else hi = mid;
-            if (c == top) break;
+            if (c == top || hi - lo <= 1) break;
+            mid = lo + (hi - lo) / 2;
         }
         __syncthreads();
         if (t == 0) s.count = 0;
@@ -454,18 +454,22 @@ token_logprobs_kernel(const T* logits, int64_t ld, int vocab, const int64_t* tok
             if ((tile & (tile - 1)) == 0 || tile % 8 == 0 || i0 + TILE >= end) {
                 __syncthreads();
                 const int n = s.n;
-                if (n <= room) {
+                if (n <= top + LP_LONG) {
+                    n_met = n;
+                    __syncthreads();                           // everyone knows n before it grows
+                } else if (n <= room) {
                     bound = meet(n, bound);
+                    n_met = top;
                 } else {                                       // too many: those tiles again, with care
                     __syncthreads();
                     if (t == 0) s.n = n_met;
                     __syncthreads();
                     for (int i = met; i <= i0; i += TILE) bound = careful(i, bound);
+                    __syncthreads();
+                    n_met = s.n;
+                    __syncthreads();
                 }
-                __syncthreads();
                 met = i0 + TILE;
-                n_met = s.n;
-                __syncthreads();
             }
         }
         stage = stage + 1 == LP_STAGES ? 0 : stage + 1;

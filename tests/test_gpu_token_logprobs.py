@@ -118,6 +118,19 @@ def test_a_token_that_is_nearly_certain(vocab, dtype):
     assert torch.equal(got.top_logprobs[:, 0], got.logprobs) and torch.equal(got.top_tokens[:, 0], at)
 
 
+@pytest.mark.parametrize("vocab", [2000, 50000])
+def test_rows_with_many_nan(vocab):
+    """NaN everywhere, at the front, in every second place: the lowest indices come first, whatever the list is cut by."""
+    x = torch.randn(3, vocab, device=DEV)
+    x[0] = math.nan
+    x[1, :1500] = math.nan
+    x[2, ::2] = math.nan
+    for top in (1, 2, 64):
+        got = few_rows.token_logprobs(x, top=top)
+        i = torch.arange(top, device=DEV)
+        assert torch.equal(got.top_tokens, torch.stack([i, i, 2 * i])) and got.top_logprobs.isnan().all() and got.entropy.isnan().all()
+
+
 def test_rows_of_other_layouts():
     big = torch.randn(40, 3001, device=DEV).bfloat16()
     tokens = torch.randint(0, 2999, (40,), device=DEV)
