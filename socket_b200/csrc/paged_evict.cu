@@ -17,9 +17,9 @@ namespace sk {
 namespace {
 
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 8;
-// Moves a thread has under way: many rows share an SM by two blocks, a cluster's are few
-template <int CL> constexpr int EV_MOVES_OF = CL == 1 ? 2 : 4;
-template <int CL> constexpr int EV_PER_SM = CL == 1 ? 2 : 1;
+// Two blocks an SM, which leaves registers for two moves a thread under way.  One block with four (4 sequences of 8 heads, 32768 to 4096 slots):
+// 79 us, as their 256 blocks then come in two turns; two blocks with two moves 43
+constexpr int EV_PER_SM = 2, EV_MOVES = 2;
 constexpr int EV_SLOTS = 24576;                                // of a block, whose keys and positions find room in shared memory
 struct alignas(16) EvMove {
     int from, to;
@@ -63,7 +63,7 @@ template <int CL> __device__ __forceinline__ void ev_sync() {
 }
 
 template <int CL>
-__global__ void __launch_bounds__(EV_THREADS, EV_PER_SM<CL>)
+__global__ void __launch_bounds__(EV_THREADS, EV_PER_SM)
 paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int recent, int sink, float* mass_out, int64_t mo_bs, int64_t mo_hs,
                    int32_t* pos_out, int64_t po_bs, int64_t po_hs, int32_t* lengths_out, EvMove* moves, int most_moves, int room) {
     pdl_begin();
@@ -289,7 +289,6 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
     ev_sync<CL>();                                             // the list is complete, and the others' counts are read
 
     // ---- moves: a thread per 16-byte piece of some of them
-    constexpr int EV_MOVES = EV_MOVES_OF<CL>;
     const int es = c.dtype == SK_F32 ? 4 : 2, pieces = c.D * es / 16, per = 1 << (32 - __clz(pieces - 1)), p = t & (per - 1);
     const int step = EV_THREADS / per, shift = 31 - __clz(c.page);
     for (int i0 = rank * EV_MOVES * step + t / per; i0 < moves_n; i0 += CL * EV_MOVES * step) {
