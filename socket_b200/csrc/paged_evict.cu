@@ -6,9 +6,10 @@
 // list entry is a row of K, a row of V, a mass and a position to move; sources lie behind the budget and targets below it, so the
 // cluster's blocks move entries in any order once the list is complete.  Only what moves is read: mass and positions once, 241 of 4352 keys of D elements.
 //
-// Measured, 8 heads of 128: 32 sequences from 4352 to 4096 slots 28 us (about 17 in four passes of three barriers each, then 63 MB of rows), one from
-// 32768 to 4096 27.7 us (15 until its moves begin: passes end in barriers of the cluster).  With the moves in a kernel of their own 31 and 28, and a
-// launch more; with three histograms of 2048 bins 29 and 52, words of other blocks cost that much.
+// Measured, 8 heads of 128: 32 sequences from 4352 to 4096 slots 26.7 us (about 14 in passes of three barriers each, then 63 MB of rows), one from
+// 32768 to 4096 25.7 us (13 until its moves begin: passes end in barriers of the cluster).  Always four passes: 28.2 and 28; list and table read when
+// a move needs them instead of a turn ahead: 26.8 and 26.8; every warp finding the digit for itself, a barrier less a pass: 27.3 and 26.9.  With the moves in
+// a kernel of their own 3 more, and a launch; with three histograms of 2048 bins 29 and 52, words of other blocks cost that much.
 #include "paged.cuh"
 
 #include <type_traits>
@@ -189,14 +190,16 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
             __syncthreads();
             prefix = prefix << 8 | s.digit;
             need = s.need;
+            if (s.equal == need) {                             // all that are left are kept, in every block of the cluster
+                prefix <<= 24 - 8 * pass;
+                break;
+            }
         }
         const bool ties = s.equal > need;                      // only some of the equal keys are kept: the first ones
 
         // ---- in slot order, a run of slots per warp: freed slots, kept slots behind the budget
         const int run = (count + EV_WARPS * 32 - 1) / (EV_WARPS * 32) * 32, i0 = min(warp * run, count), i1 = min(i0 + run, count);
-        auto before = [&](int which, int mine, int& all) {     // sum over the warps in front; `all`: over the block
-            if (lane == 0) s.part[which][warp] = mine;
-            __syncthreads();
+        auto before = [&](int which, int& all) {               // sum over the warps in front; `all`: over the block
             const int x = lane < EV_WARPS ? s.part[which][lane] : 0;
             all = __reduce_add_sync(FULL, x);
             return __reduce_add_sync(FULL, lane < warp ? x : 0);
@@ -205,7 +208,9 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         if (ties) {
             int equal = 0;
             for (int i = i0 + lane; i - lane < i1; i += 32) equal += __popc(__ballot_sync(FULL, i < i1 && key(i) == prefix));
-            equal_at = before(0, equal, all);
+            if (lane == 0) s.part[0][warp] = equal;
+            __syncthreads();
+            equal_at = before(0, all);
             if constexpr (CL > 1) {
                 if (t == 0) s.equals = all;
                 ev_sync<CL>();
@@ -233,7 +238,12 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
         }
         holes = __reduce_add_sync(FULL, holes);
         movers = __reduce_add_sync(FULL, movers);
-        int all_holes, all_movers, hole_at = before(1, holes, all_holes), mover_at = before(2, movers, all_movers);
+        if (lane == 0) {
+            s.part[1][warp] = holes;
+            s.part[2][warp] = movers;
+        }
+        __syncthreads();
+        int all_holes, all_movers, hole_at = before(1, all_holes), mover_at = before(2, all_movers);
         if constexpr (CL > 1) {
             if (t == 0) {
                 s.holes = all_holes;
@@ -291,18 +301,30 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
     // ---- moves: a thread per 16-byte piece of some of them
     const int es = c.dtype == SK_F32 ? 4 : 2, pieces = c.D * es / 16, per = 1 << (32 - __clz(pieces - 1)), p = t & (per - 1);
     const int step = EV_THREADS / per, shift = 31 - __clz(c.page);
-    for (int i0 = rank * EV_MOVES * step + t / per; i0 < moves_n; i0 += CL * EV_MOVES * step) {
-        int4 e[EV_MOVES];
-        int from[EV_MOVES], to[EV_MOVES];
+    int4 next[EV_MOVES];
+    int next_from[EV_MOVES], next_to[EV_MOVES];
+    auto fetch = [&](int i0) {                                 // of the list and the table, a turn ahead
 #pragma unroll
         for (int x = 0; x < EV_MOVES; ++x)
-            if (i0 + x * step < moves_n) e[x] = __ldcg(reinterpret_cast<const int4*>(list + i0 + x * step));
+            if (i0 + x * step < moves_n) next[x] = __ldcg(reinterpret_cast<const int4*>(list + i0 + x * step));
 #pragma unroll
         for (int x = 0; x < EV_MOVES; ++x)
             if (i0 + x * step < moves_n) {
-                from[x] = __ldcg(c.table + b * c.table_ld + (e[x].x >> shift));
-                to[x] = __ldcg(c.table + b * c.table_ld + (e[x].y >> shift));
+                next_from[x] = __ldcg(c.table + b * c.table_ld + (next[x].x >> shift));
+                next_to[x] = __ldcg(c.table + b * c.table_ld + (next[x].y >> shift));
             }
+    };
+    const int first = rank * EV_MOVES * step + t / per;
+    fetch(first);
+    for (int i0 = first; i0 < moves_n; i0 += CL * EV_MOVES * step) {
+        int4 e[EV_MOVES];
+        int from[EV_MOVES], to[EV_MOVES];
+#pragma unroll
+        for (int x = 0; x < EV_MOVES; ++x) {
+            e[x] = next[x];
+            from[x] = next_from[x];
+            to[x] = next_to[x];
+        }
         uint4 k[EV_MOVES], v[EV_MOVES];
         bool ok[EV_MOVES];
 #pragma unroll
@@ -314,6 +336,7 @@ paged_evict_kernel(const __grid_constant__ sk_paged_cache c, int budget, int rec
                 v[x] = __ldcs(reinterpret_cast<const uint4*>((const char*)c.v + (from[x] * c.v_ps + g * c.v_hs + r * c.v_rs) * es) + p);
             }
         }
+        fetch(i0 + CL * EV_MOVES * step);
 #pragma unroll
         for (int x = 0; x < EV_MOVES; ++x) {
             if (i0 + x * step >= moves_n) continue;

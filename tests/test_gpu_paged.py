@@ -376,6 +376,24 @@ def test_evict_long(n, budget, fill):
     _evict_case([n, n // 2], 2, 8, 64, torch.bfloat16, budget, min(100, budget // 2), 1, fill)
 
 
+@pytest.mark.parametrize("n,over", [(600, 0), (600, 1), (600, -1), (20000, 0), (20000, 1), (20000, -1)])
+@pytest.mark.parametrize("byte", [3, 2, 1, 0])
+@pytest.mark.parametrize("base", [0x00000000, 0x3E123455])
+def test_evict_cut_between_bytes(base, byte, n, over):
+    """Two masses that differ in one byte, the larger ones as many as the budget, one more or one fewer."""
+    c = Cache([n], 2, 8, 64, torch.bfloat16, DEV, seed=byte)
+    g = torch.Generator(device=DEV).manual_seed(byte)
+    large = torch.rand(1, 2, c.cap, generator=g, device=DEV).argsort(-1) < n // 3
+    large[..., n:] = False
+    budget = int(large[0, 0].sum()) - over
+    bits = torch.where(large, base + (1 << 8 * byte), base).to(torch.int32)
+    mass = bits.view(torch.float32)
+    positions = torch.arange(c.cap, device=DEV, dtype=torch.int32).expand(1, 2, c.cap).contiguous()
+    k, v = c.k.clone(), c.v.clone()
+    got = paged.evict(c.k, c.v, c.table, c.lengths, mass.clone(), positions.clone(), budget=budget)
+    _check_evict(c, [n], mass, positions, budget, 0, 0, got, k, v)
+
+
 def test_evictions_captured_and_replayed():
     """A graph that collects weights and cuts in place, replayed: the same as eager calls on copies."""
     c = Cache([200, 90, 131], 2, 64, 16, torch.bfloat16, DEV, room=40)
