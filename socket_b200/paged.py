@@ -134,6 +134,7 @@ def attn(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Te
     assert out.shape == shape and out.dtype == q.dtype and os[2] == 1
     entry = lib()
     need = entry.sk_paged_attn_workspace_bytes(c, H)
+    assert workspace is None or workspace.is_contiguous()
     have = 0 if workspace is None else workspace.numel() * workspace.element_size()
     if have < need:
         workspace, have = torch.empty(need, dtype=torch.uint8, device=q.device), need

@@ -229,6 +229,28 @@ def test_attention_with_its_own_workspace():
         assert torch.equal(paged.attn(q, *c.tensors, mass=m2, workspace=ws), out) and torch.equal(m2, m)
 
 
+def test_refused_tensors():
+    c = Cache([40, 9], 2, 64, 16, torch.float16, DEV)
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    mass, pos = torch.zeros(2, 2, c.cap, device=DEV), torch.zeros(2, 2, c.cap, dtype=torch.int32, device=DEV)
+    need = 65536                                              # without weights so short a batch needs none: an empty one would be contiguous
+    for ws in (torch.zeros(1, dtype=torch.uint8, device=DEV).expand(need), torch.zeros(2 * need, dtype=torch.uint8, device=DEV)[::2]):
+        with pytest.raises(AssertionError):                    # fewer bytes, or others, than it counts
+            paged.attn(q, *c.tensors, workspace=ws)
+    for refused in (lambda: paged.attn(q.float(), *c.tensors), lambda: paged.attn(q[:1], *c.tensors), lambda: paged.attn(q[:, :3], *c.tensors),
+                    lambda: paged.attn(q, *c.tensors, mass=mass[..., :-1]), lambda: paged.attn(q, *c.tensors, mass=mass.double()),
+                    lambda: paged.attn(q, c.k, c.v, c.table.long(), c.lengths), lambda: paged.attn(q, c.k, c.v, c.table, c.lengths[:1]),
+                    lambda: paged.append(q[:, None], q[:, None], *c.tensors), lambda: paged.evict(*c.tensors, mass, pos.long(), budget=8),
+                    lambda: paged.evict(*c.tensors, mass, pos, budget=8, out=(mass, pos, c.lengths.long()))):
+        with pytest.raises(AssertionError):
+            refused()
+    for refused in (lambda: paged.evict(*c.tensors, mass, pos, budget=0), lambda: paged.attn(q, *c.tensors, extra=-1)):
+        with pytest.raises(_lib.SocketError):
+            refused()
+    with pytest.raises(RuntimeError):
+        paged.attn(q.cpu(), *c.tensors)
+
+
 def test_two_captured_steps_that_replay_together():
     """Two graphs of append and attention on two streams, replayed while lengths grow: every replay is a fresh call's result."""
     caches = [Cache([600, 31], 2, 64, 16, torch.bfloat16, DEV, room=8, seed=i) for i in range(2)]
