@@ -17,7 +17,7 @@
 namespace sk {
 namespace {
 
-constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 8;
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 16;
 // Two blocks an SM, which leaves registers for two moves a thread under way.  One block with four (4 sequences of 8 heads, 32768 to 4096 slots):
 // 79 us, as their 256 blocks then come in two turns; two blocks with two moves 43
 constexpr int EV_PER_SM = 2, EV_MOVES = 2;
@@ -369,10 +369,12 @@ struct EvPlan {
 EvPlan ev_plan(const sk_paged_cache& c, int budget) {
     EvPlan p;
     const int64_t rows = (int64_t)c.B * c.G, cap = (int64_t)c.width * c.page;
-    // blocks of a row: while they find a place at once, two an SM, and have four slots a thread; more where its slots have no room on chip
+    // Blocks of a row: twice as many while they find a place at once, two an SM, and then have four slots a thread, eight where they are 16 (one row of
+    // 65536 slots 26 us by 16 and 34 by 8, eight of 32768 29 and 26); more where a block's slots have no room on chip
     p.cluster = 1;
-    while (p.cluster < EV_CLUSTER && ((rows * 2 * p.cluster <= 2 * sm_count() && cap >= (int64_t)8 * EV_THREADS * p.cluster) ||
-                                      (cap + p.cluster - 1) / p.cluster > EV_SLOTS))
+    while (p.cluster < EV_CLUSTER &&
+           ((rows * 2 * p.cluster <= 2 * sm_count() && cap >= (int64_t)(p.cluster < 8 ? 8 : 16) * EV_THREADS * p.cluster) ||
+            (cap + p.cluster - 1) / p.cluster > EV_SLOTS))
         p.cluster *= 2;
     const int64_t share = (cap + p.cluster - 1) / p.cluster;
     p.room = (int)(share < EV_SLOTS ? share : EV_SLOTS);
@@ -388,6 +390,10 @@ int evict_launch(const sk_paged_cache& c, int budget, int recent, int sink, floa
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)paged_evict_kernel<CL>, (size_t)EV_SLOTS * 8);
     if (e != cudaSuccess) return check_chained(e, "paged_evict_kernel");
+    if (CL > 8) {                                              // more than every GPU takes
+        e = cudaFuncSetAttribute((const void*)paged_evict_kernel<CL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return check_chained(e, "paged_evict_kernel");
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(c.B * c.G * CL));
     cfg.blockDim = dim3(EV_THREADS);
@@ -414,7 +420,7 @@ int launch_paged_evict(const sk_paged_cache& c, int budget, int recent, int sink
     const EvPlan p = ev_plan(c, budget);
     if ((int64_t)c.B * c.G * EV_CLUSTER > INT32_MAX) return fail(SK_ERR_UNSUPPORTED, "sk_paged_evict: %d sequences with %d heads", c.B, c.G);
     const bool apart = lengths_out + c.B <= c.lengths || c.lengths + c.B <= lengths_out;
-    auto go = p.cluster == 8 ? evict_launch<8> : p.cluster == 4 ? evict_launch<4> : p.cluster == 2 ? evict_launch<2> : evict_launch<1>;
+    auto go = p.cluster == 16 ? evict_launch<16> : p.cluster == 8 ? evict_launch<8> : p.cluster == 4 ? evict_launch<4> : p.cluster == 2 ? evict_launch<2> : evict_launch<1>;
     if (int rc = go(c, budget, recent, sink, mass_out, mo_bs, mo_hs, pos_out, po_bs, po_hs, apart ? lengths_out : nullptr, (EvMove*)workspace, p, st))
         return rc;
     if (apart) return SK_OK;

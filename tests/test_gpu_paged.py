@@ -358,8 +358,8 @@ def _check_evict(c, lengths, mass, positions, budget, recent, sink, got, k_befor
     assert torch.equal(c.v.contiguous().view(bits), want_v.contiguous().view(bits))
 
 
-def _evict_case(lengths, G, D, page, dtype, budget, recent, sink, fill, seed=0, in_place=False, combined=False):
-    c = Cache(lengths, G, D, page, dtype, DEV, seed=seed, combined=combined)
+def _evict_case(lengths, G, D, page, dtype, budget, recent, sink, fill, seed=0, in_place=False, combined=False, room=0):
+    c = Cache(lengths, G, D, page, dtype, DEV, seed=seed, combined=combined, room=room)
     g = torch.Generator(device=DEV).manual_seed(seed + 1)
     shape = (len(lengths), G, c.cap)
     mass = {"random": lambda: torch.rand(shape, generator=g, device=DEV), "equal": lambda: torch.full(shape, 0.25, device=DEV),
@@ -396,6 +396,15 @@ def test_evict_layouts(G, D, page, dtype, combined):
 @pytest.mark.parametrize("fill", ["random", "few"])
 def test_evict_long(n, budget, fill):
     _evict_case([n, n // 2], 2, 8, 64, torch.bfloat16, budget, min(100, budget // 2), 1, fill)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lengths,budget", [([410000, 7], 100000), ([400, 70000] + [3] * 22, 350)])
+@pytest.mark.parametrize("fill", ["random", "few"])
+def test_evict_slots_without_room_on_chip(lengths, budget, fill, in_place):
+    """More slots than sixteen blocks hold; more sequences than find a place at once, with tables as wide."""
+    room = max(0, 200000 - max(lengths))
+    _evict_case(lengths, 1, 8, 64, torch.bfloat16, budget, 100, 1, fill, in_place=in_place, room=room)
 
 
 @pytest.mark.parametrize("n,over", [(600, 0), (600, 1), (600, -1), (20000, 0), (20000, 1), (20000, -1)])
