@@ -22,6 +22,7 @@ constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 16;
 // 79 us, as their 256 blocks then come in two turns; two blocks with two moves 43
 constexpr int EV_PER_SM = 2, EV_MOVES = 2;
 constexpr int EV_SLOTS = 24576;                                // of a block, whose keys and positions find room in shared memory
+constexpr int EV_SLOTS_OF_TWO = 13824;                         // where two blocks share an SM
 struct alignas(16) EvMove {
     int from, to;
     float mass;
@@ -369,13 +370,17 @@ struct EvPlan {
 EvPlan ev_plan(const sk_paged_cache& c, int budget) {
     EvPlan p;
     const int64_t rows = (int64_t)c.B * c.G, cap = (int64_t)c.width * c.page;
-    // Blocks of a row: twice as many while they find a place at once, two an SM, and then have four slots a thread, eight where they are 16 (one row of
-    // 65536 slots 26 us by 16 and 34 by 8, eight of 32768 29 and 26); more where a block's slots have no room on chip
+    // Blocks of a row: twice as many while they find a place at once, two an SM, and then have four slots a thread; more where a block's slots have no
+    // room on chip.  Sixteen come later, with eight slots a thread (one row of 65536 slots 26 us by 16 and 34 by 8, eight of 32768 29 and 26), and for
+    // more rows than half fill the GPU only where eight would not share SMs (16 rows of 131072 slots 192 and 281, of 70000 117 and 104)
     p.cluster = 1;
-    while (p.cluster < EV_CLUSTER &&
-           ((rows * 2 * p.cluster <= 2 * sm_count() && cap >= (int64_t)(p.cluster < 8 ? 8 : 16) * EV_THREADS * p.cluster) ||
-            (cap + p.cluster - 1) / p.cluster > EV_SLOTS))
+    while (p.cluster < EV_CLUSTER) {
+        const bool find_places = rows * 2 * p.cluster <= 2 * sm_count(), sixteen = p.cluster == 8;
+        const bool pays = !sixteen ? cap >= (int64_t)8 * EV_THREADS * p.cluster
+                                   : cap >= (int64_t)16 * EV_THREADS * 8 && (rows * 16 <= sm_count() || cap > (int64_t)EV_SLOTS_OF_TWO * 8);
+        if (!(find_places && pays) && (cap + p.cluster - 1) / p.cluster <= EV_SLOTS) break;
         p.cluster *= 2;
+    }
     const int64_t share = (cap + p.cluster - 1) / p.cluster;
     p.room = (int)(share < EV_SLOTS ? share : EV_SLOTS);
     const int64_t behind = cap > budget ? cap - budget : 0;
