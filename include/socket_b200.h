@@ -483,7 +483,8 @@ SK_API int sk_paged_append(const sk_paged_cache* c, const void* k_new, int64_t k
 
 /* Softmax attention of one query token per sequence, q [B, H, D] (heads q_hs, sequences q_bs apart; H a multiple of G,
  * query heads of one key/value head in a row), over the first lengths[b] + extra slots: out [B, H, D] in q's type (that of
- * the pools), scores scale * q.k, all sums in fp32.  No key: zeros.  With mass, every attended slot of (b, g) is increased by
+ * the pools), scores scale * q.k, all sums in fp32; for 16-bit pools a weight enters its products with 16 bits, however small it is
+ * beside others, and an infinite value among the attended ones gives infinity or NaN.  No key: zeros.  With mass, every attended slot of (b, g) is increased by
  * the sum of its weights over the query heads of g.  No atomics: the result does not depend on the order blocks run in.
  * `workspace`: sk_paged_attn_workspace_bytes of the same cache and H, overwritten by every call. */
 SK_API size_t sk_paged_attn_workspace_bytes(const sk_paged_cache* c, int H);

@@ -17,7 +17,8 @@
 //
 // 16-bit types: S^T = K Q^T and O^T = V^T P^T by m16n8k16 products, keys and then value columns in the 16 rows and up to 8 query heads in
 // the 8 columns, which wastes half of what heads in the rows would.  Weights go in as two halves (value and rounding rest), so that what is
-// added up has 16 bits of each weight.  fp32: fused multiply-adds, a lane per key for scores, a lane per four columns for values.
+// added up has 16 bits of each weight.  In fp16 both halves end at 2^-24: its reference stands below the maximum, so that weights reach 2^15, and those
+// under 2^-9 go in by themselves, multiplied by 2^24.  fp32: fused multiply-adds, a lane per key for scores, a lane per four columns for values.
 #include "paged.cuh"
 #include "warp_mma.cuh"
 
@@ -29,6 +30,10 @@ constexpr int PT_KEYS = 16;                                    // keys of a warp
 // A running maximum is only raised for a score this far (in powers of two) above it: weights then reach 2^8, which neither a half nor
 // the sums mind, and the six exchanges and the rescaling that a rise takes are left out of nearly every tile.
 constexpr float PT_SLACK = 8.f;
+// fp16: raised to PT16_BELOW under the maximum, for a score PT16_SLACK above that.  Weights then reach 2^15 of a largest half of 65504, and only those
+// 20 powers of two under a maximum are small.  64 sequences of 1 to 8003 with mass 59.4 us, 58.0 with small weights lost; 4 x 131072 keys 348, of which
+// all but one are small 373, and 397 where they take two turns (344, all lost)
+constexpr float PT16_BELOW = 11.f, PT16_SLACK = 4.f, PT16_SMALL = 0x1p-9f, PT16_UP = 0x1p24f;
 
 template <typename T, int DP_, int NT_> struct PtShape {
     static constexpr int DP = DP_, NT = NT_;                   // head size padded, groups of heads
@@ -278,6 +283,7 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
 
     // ---- queries of a pair, running maxima and sums
     constexpr int KK = DP / 16, NT = S::NT;
+    constexpr bool NARROW = std::is_same_v<T, __half>;         // a type whose smallest weights need care
     constexpr int CPL = S::F32 ? (DP / 4 + 31) / 32 : 1;       // fp32: 16-byte pieces of a value row per lane
     uint32_t qf[S::F32 ? 1 : NT][S::F32 ? 1 : KK][2];
     float acc[S::F32 ? HG : KK][S::F32 ? CPL : NT][4];         // 16 bit: rows of value columns x heads; fp32: heads x columns
@@ -360,7 +366,7 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                         if ((lane >> 2) + 8 < rows) __stcg(reinterpret_cast<float2*>(o + 8 * a.rs), make_float2(s[nt][2], s[nt][3]));
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) above |= fmaxf(s[nt][i], s[nt][i + 2]) > m[nt * 2 + i] + PT_SLACK;
+                    for (int i = 0; i < 2; ++i) above |= fmaxf(s[nt][i], s[nt][i + 2]) - m[nt * 2 + i] > (NARROW ? PT16_BELOW + PT16_SLACK : PT_SLACK);
                 }
                 if (__any_sync(FULL, above)) {                 // maxima follow, and what was summed up with them
 #pragma unroll
@@ -369,6 +375,7 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                         mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 16));
+                        if (NARROW) mx = __fsub_ru(mx, PT16_BELOW);            // of huge scores too no more than this below
                         const float mn = fmaxf(m[x], mx), f = pt_factor(m[x], mn);
                         m[x] = mn;
                         l[x] *= f;
@@ -380,6 +387,17 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                     }
                 }
                 uint32_t ph[NT][2], pl[NT][2];
+                auto halves = [&](const float (&w)[NT][4]) {   // keys x heads of a lane's row to those of its column
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t h = pt_pack<T>(w[nt][2 * i], w[nt][2 * i + 1]);
+                            ph[nt][i] = pt_turn(h);
+                            pl[nt][i] = pt_turn(pt_pack<T>(w[nt][2 * i] - pt_low<T>(h), w[nt][2 * i + 1] - pt_high<T>(h)));
+                        }
+                };
+                float least = PT16_SMALL;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -388,15 +406,51 @@ paged_attn_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                         s[nt][i] = exp2_fast(s[nt][i] - mc);
                         s[nt][i + 2] = exp2_fast(s[nt][i + 2] - mc);
                         l[nt * 2 + i] += s[nt][i] + s[nt][i + 2];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t h = pt_pack<T>(s[nt][2 * i], s[nt][2 * i + 1]);
-                        ph[nt][i] = pt_turn(h);
-                        pl[nt][i] = pt_turn(pt_pack<T>(s[nt][2 * i] - pt_low<T>(h), s[nt][2 * i + 1] - pt_high<T>(h)));
+                        if (NARROW) least = fminf(least, fminf(s[nt][i], s[nt][i + 2]));
                     }
                 }
                 const uint32_t vrow = saddr(vt) + ((lane & 7) + (lane >> 4) * 8) * S::ROW + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
+                if constexpr (NARROW) {
+                    if (__any_sync(FULL, least < PT16_SMALL)) {                // 24 powers of two at a time
+                        float rest[NT][4];
+#pragma unroll
+                        for (int i = 0; i < 4 * NT; ++i) {
+                            float& w = (&s[0][0])[i];
+                            (&rest[0][0])[i] = w < PT16_SMALL ? w : 0.f;
+                            w = w < PT16_SMALL ? 0.f : w;
+                        }
+                        float down = 1.f;
+                        bool small;
+                        do {
+                            float w[NT][4];
+                            down /= PT16_UP;
+                            small = false;
+#pragma unroll
+                            for (int i = 0; i < 4 * NT; ++i) {
+                                float& r = (&rest[0][0])[i];
+                                r *= PT16_UP;
+                                (&w[0][0])[i] = r < PT16_SMALL ? 0.f : r;
+                                r = r < PT16_SMALL ? r : 0.f;
+                                small |= r > 0.f;
+                            }
+                            halves(w);
+#pragma unroll
+                            for (int mt = 0; mt < KK; ++mt) {
+                                uint32_t v4[4];
+                                ldsm4t(vrow ^ (mt << 5), v4);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma16816(sum, v4[0], v4[1], v4[2], v4[3], ph[nt][0], ph[nt][1], (const T*)nullptr);
+                                    mma16816(sum, v4[0], v4[1], v4[2], v4[3], pl[nt][0], pl[nt][1], (const T*)nullptr);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) acc[mt][nt][e] = fmaf(sum[e], down, acc[mt][nt][e]);
+                                }
+                            }
+                        } while (__any_sync(FULL, small));
+                    }
+                }
+                halves(s);
 #pragma unroll
                 for (int mt = 0; mt < KK; ++mt) {
                     uint32_t v4[4];
