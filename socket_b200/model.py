@@ -370,7 +370,8 @@ class Transformer(Decoder):
         self.norm = RMSNorm(config.dim, eps=config.norm_eps)
         self.output = nn.Linear(config.dim, config.vocab_size, bias=False)
         self.register_buffer("freqs_cis", None, persistent=False)
-        self.paging: Optional[Paging] = None
+        self.chosen_paging: Optional[Paging] = None           # by `use_pages`
+        self.paging: Optional[Paging] = None                  # of the caches that are there or come next
         self.pages: Optional[PageTable] = None
         self.tp_fused = True                       # decode: fuse wo / w2 with the sum over the ranks (GPU, <= 8 rows)
         self._fused_sum = None
@@ -409,19 +410,26 @@ class Transformer(Decoder):
             dst.copy_(tensors[name])
 
     def use_pages(self, paging: Optional[Paging] = Paging()) -> "Transformer":
-        """Keep the caches in pages (None: in one piece per sequence again) and decode with mode "paged".  Caches that are
-        there are dropped: `setup_caches` and `setup_decode` follow."""
-        self.paging, self.pages = paging, None
+        """Keep the caches in pages (None: in one piece per sequence again) and decode with mode "paged" where no other is asked
+        for.  Caches that are there are dropped: `setup_caches` and `setup_decode` follow."""
+        self.chosen_paging = paging
         self.default_mode = type(self).default_mode if paging is None else "paged"
+        self._keep_caches(paging)
+        return self
+
+    def _keep_caches(self, paging: Optional[Paging]) -> None:
+        """Drops the caches; those that `setup_caches` makes are kept by `paging`."""
+        self.paging, self.pages = paging, None
         self.release_decode()
         self.max_batch_size = self.max_seq_length = -1
         for layer in self.layers:
             layer.attention.kv_cache = layer.attention.workspace = None
-        return self
 
     def choose_mode(self, mode: Optional[str]) -> None:
-        if mode is not None and (mode == "paged") != (self.paging is not None):
-            self.use_pages(Paging() if mode == "paged" else None)
+        """Caches in pages for mode "paged", as `use_pages` chose them, else in one piece; what was chosen stays."""
+        paged = (self.default_mode if mode is None else mode) == "paged"
+        if paged != (self.paging is not None):
+            self._keep_caches((self.chosen_paging or Paging()) if paged else None)
 
     def setup_caches(self, max_batch_size: int, max_seq_length: int) -> None:
         if self.pages is not None and max_batch_size != self.pages.table.shape[0]:
@@ -488,6 +496,7 @@ class Transformer(Decoder):
     def setup_decode(self, batch: int, mode: Optional[str] = None, use_graph: bool = True) -> None:
         if self.pages is None:
             return super().setup_decode(batch, mode, use_graph)
+        mode = "paged" if mode is None else mode                # a call's mode may have made these caches
         if batch != self.pages.table.shape[0]:
             raise RuntimeError(f"{batch} sequences on caches in pages for {self.pages.table.shape[0]}")
         counters = self.pages.counters.clone()
