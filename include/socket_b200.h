@@ -460,6 +460,7 @@ SK_API int sk_begin_token(const int64_t* first, int64_t* token, int batch, int64
  * mass_hs / pos_hs and sequences mass_bs / pos_bs elements apart.
  * page is a power of two, at least 16; D a multiple of 8 (bf16, fp16) or 4 (fp32), at most 256.  Pools and their strides
  * are 16-byte aligned, rows less than 2^29 elements apart.  Sequences may share pages that are only read; a page that a call writes belongs to one sequence.
+ * What a call writes shares no element with itself: each of its dimensions lies inside the next larger stride's.
  * A slot behind the last is not touched (SK_DEV_POS_OUT_OF_RANGE), nor is a page outside [0, n_pages)
  * (SK_DEV_INDEX_OUT_OF_RANGE): its keys are left out. */
 typedef struct sk_paged_cache {

@@ -1,6 +1,8 @@
 // Entry points of the paged cache, and the append that fills its pages.
 #include "paged.cuh"
 
+#include <algorithm>
+
 namespace sk {
 namespace {
 
@@ -103,6 +105,33 @@ int paged_check(const sk_paged_cache* c, const char* what) {
     return SK_OK;
 }
 
+namespace {
+
+// Rows of `inner` elements, n of them s elements apart in every one of three dimensions: no two share an element, where one
+// dimension lies inside the other.  What a call writes; what it reads may be expanded.
+struct PagedDim {
+    int64_t n, s;
+};
+bool paged_apart(int64_t inner, PagedDim a, PagedDim b, PagedDim c = {1, 0}) {
+    PagedDim d[3] = {a, b, c};
+    std::sort(d, d + 3, [](const PagedDim& x, const PagedDim& y) { return x.s < y.s; });
+    __int128 extent = inner;
+    for (const PagedDim& x : d) {
+        if (x.n == 0) return true;
+        if (x.n == 1) continue;
+        if (x.s < extent) return false;
+        extent += (__int128)x.s * (x.n - 1);
+    }
+    return true;
+}
+bool paged_book_apart(const sk_paged_cache& c, int64_t bs, int64_t hs) {
+    return paged_apart((int64_t)c.width * c.page, {c.B, bs}, {c.G, hs});
+}
+bool paged_pools_apart(const sk_paged_cache& c) {
+    return paged_apart(c.D, {c.n_pages, c.k_ps}, {c.G, c.k_hs}, {c.page, c.k_rs}) && paged_apart(c.D, {c.n_pages, c.v_ps}, {c.G, c.v_hs}, {c.page, c.v_rs});
+}
+
+}  // namespace
 }  // namespace sk
 
 using namespace sk;
@@ -118,6 +147,8 @@ int sk_paged_append(const sk_paged_cache* c, const void* k_new, int64_t kn_bs, i
     const int v = 16 / (int)esize(c->dtype);
     if (!aligned(k_new, 16) || !aligned(v_new, 16) || kn_bs % v || kn_ss % v || kn_hs % v || vn_bs % v || vn_ss % v || vn_hs % v)
         return fail(SK_ERR_MISALIGNED, "sk_paged_append: new rows and their strides must be 16-byte aligned");
+    SK_REQUIRE(paged_pools_apart(*c) && (c->mass == nullptr || paged_book_apart(*c, c->mass_bs, c->mass_hs)) &&
+               (c->positions == nullptr || paged_book_apart(*c, c->pos_bs, c->pos_hs)), "sk_paged_append: rows of pools, mass or positions overlap");
     return launch_paged_append(*c, k_new, kn_bs, kn_ss, kn_hs, v_new, vn_bs, vn_ss, vn_hs, S, counts, first, (cudaStream_t)stream);
 }
 
@@ -135,6 +166,8 @@ int sk_paged_attn(const sk_paged_cache* c, const void* q, int64_t q_bs, int64_t 
     const int v = 16 / (int)esize(c->dtype);
     if (!aligned(q, 16) || !aligned(out, 16) || q_bs % v || q_hs % v || o_bs % v || o_hs % v)
         return fail(SK_ERR_MISALIGNED, "sk_paged_attn: q, out and their strides must be 16-byte aligned");
+    SK_REQUIRE(paged_apart(c->D, {c->B, o_bs}, {H, o_hs}) && (c->mass == nullptr || paged_book_apart(*c, c->mass_bs, c->mass_hs)),
+               "sk_paged_attn: rows of out or mass overlap");
     const size_t need = paged_attn_workspace(*c, H);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(SK_ERR_WORKSPACE, "sk_paged_attn: workspace of %zu bytes, %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
@@ -154,6 +187,8 @@ int sk_paged_evict(const sk_paged_cache* c, int budget, int recent, int sink, fl
                budget, sink, recent);
     if (c->B == 0) return SK_OK;
     SK_REQUIRE(lengths_out && (c->width == 0 || (c->mass && c->positions && mass_out && pos_out)), "sk_paged_evict: null pointer");
+    SK_REQUIRE(paged_pools_apart(*c) && paged_book_apart(*c, mo_bs, mo_hs) && paged_book_apart(*c, po_bs, po_hs),
+               "sk_paged_evict: rows of pools, mass_out or pos_out overlap");
     const size_t need = paged_evict_workspace(*c, budget);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(SK_ERR_WORKSPACE, "sk_paged_evict: workspace of %zu bytes, %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);

@@ -4,7 +4,8 @@ a sequence within a budget.
 Pools `k_pages`, `v_pages` [pages, G, page, D] hold rows of all sequences; slot j of sequence b is row j % page of page
 `table[b, j // page]`, and `lengths[b]` slots are in use.  `mass` [B, G, slots] collects the attention weight every cached key
 gets, `positions` [B, G, slots] tells which token a slot holds: after an eviction slots are no longer in the order of tokens,
-and differ from head to head.  Attention needs neither order nor positions.
+and differ from head to head.  Attention needs neither order nor positions.  What a call only reads may be expanded; what it writes
+must not (an error).
 
 Nothing here synchronises with the host, and nothing has a CPU path.
 """
