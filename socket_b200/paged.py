@@ -216,7 +216,10 @@ class PageTable:
 
     def _show(self) -> None:
         rows = [held + [-1] * (self.width - len(held)) for held in self.held]
-        self.table.copy_(torch.tensor(rows, dtype=torch.int32).view(self.table.shape))
+        rows = torch.tensor(rows, dtype=torch.int32).view(self.table.shape)
+        if self.table.is_cuda:                                # from pinned memory the host does not wait; it is not used again before it is read
+            rows = rows.pin_memory()
+        self.table.copy_(rows, non_blocking=True)
 
     def hide(self) -> None:
         """The device sees no pages until `show`: calls on the cache then write and read nothing."""
