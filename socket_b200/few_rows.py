@@ -138,6 +138,7 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     (rows, vocab), (ld, inner) = logits.shape, logits.stride()
     if not 0 <= top <= min(TOP_TOKENS, vocab):
         raise RuntimeError(f"token_logprobs: {top} alternatives of {vocab} tokens (at most {TOP_TOKENS})")
+    assert status is None or status.dtype == torch.int32 and status.numel() == 1
     if inner != 1 or ld < vocab:
         logits = _separate_rows(logits)                           # lives until the launch
         ld = _ld(logits)
