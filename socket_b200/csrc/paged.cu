@@ -86,6 +86,19 @@ int launch_paged_append(const sk_paged_cache& c, const void* k_new, int64_t kn_b
     return SK_OK;
 }
 
+namespace {
+
+struct PagedDim {
+    int64_t n, s;                                              // entries, elements from one to the next
+};
+// Rows begin on 16-byte boundaries: v elements are 16 bytes.  The stride of one entry says nothing.
+bool paged_aligned(const void* p, int v, PagedDim a, PagedDim b, PagedDim c = {1, 0}) {
+    auto on = [v](const PagedDim& x) { return x.n <= 1 || x.s % v == 0; };
+    return aligned(p, 16) && on(a) && on(b) && on(c);
+}
+
+}  // namespace
+
 // What every call asks of a cache
 int paged_check(const sk_paged_cache* c, const char* what) {
     SK_REQUIRE(c != nullptr, "%s: null cache", what);
@@ -98,7 +111,8 @@ int paged_check(const sk_paged_cache* c, const char* what) {
     SK_REQUIRE(c->table_ld >= c->width || c->B == 1, "%s: table rows overlap", what);
     const int v = 16 / (int)esize(c->dtype);
     if (c->D % v != 0 || c->D > 256) return fail(SK_ERR_UNSUPPORTED, "%s: head size %d", what, c->D);
-    if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->k_ps % v || c->k_hs % v || c->k_rs % v || c->v_ps % v || c->v_hs % v || c->v_rs % v)
+    if (!paged_aligned(c->k, v, {c->n_pages, c->k_ps}, {c->G, c->k_hs}, {c->page, c->k_rs}) ||
+        !paged_aligned(c->v, v, {c->n_pages, c->v_ps}, {c->G, c->v_hs}, {c->page, c->v_rs}))
         return fail(SK_ERR_MISALIGNED, "%s: pools and their strides must be 16-byte aligned", what);
     // the offset of a page's row is a product of 32-bit numbers
     if (c->k_rs < 0 || c->v_rs < 0 || c->k_rs > INT32_MAX / 4 || c->v_rs > INT32_MAX / 4) return fail(SK_ERR_UNSUPPORTED, "%s: row strides", what);
@@ -109,9 +123,6 @@ namespace {
 
 // Rows of `inner` elements, n of them s elements apart in every one of three dimensions: no two share an element, where one
 // dimension lies inside the other.  What a call writes; what it reads may be expanded.
-struct PagedDim {
-    int64_t n, s;
-};
 bool paged_apart(int64_t inner, PagedDim a, PagedDim b, PagedDim c = {1, 0}) {
     PagedDim d[3] = {a, b, c};
     std::sort(d, d + 3, [](const PagedDim& x, const PagedDim& y) { return x.s < y.s; });
@@ -145,7 +156,7 @@ int sk_paged_append(const sk_paged_cache* c, const void* k_new, int64_t kn_bs, i
     if (c->B == 0 || S == 0) return SK_OK;
     SK_REQUIRE(k_new && v_new, "sk_paged_append: null pointer");
     const int v = 16 / (int)esize(c->dtype);
-    if (!aligned(k_new, 16) || !aligned(v_new, 16) || kn_bs % v || kn_ss % v || kn_hs % v || vn_bs % v || vn_ss % v || vn_hs % v)
+    if (!paged_aligned(k_new, v, {c->B, kn_bs}, {S, kn_ss}, {c->G, kn_hs}) || !paged_aligned(v_new, v, {c->B, vn_bs}, {S, vn_ss}, {c->G, vn_hs}))
         return fail(SK_ERR_MISALIGNED, "sk_paged_append: new rows and their strides must be 16-byte aligned");
     SK_REQUIRE(paged_pools_apart(*c) && (c->mass == nullptr || paged_book_apart(*c, c->mass_bs, c->mass_hs)) &&
                (c->positions == nullptr || paged_book_apart(*c, c->pos_bs, c->pos_hs)), "sk_paged_append: rows of pools, mass or positions overlap");
@@ -164,7 +175,7 @@ int sk_paged_attn(const sk_paged_cache* c, const void* q, int64_t q_bs, int64_t 
     if (c->B == 0) return SK_OK;
     SK_REQUIRE(q && out, "sk_paged_attn: null pointer");
     const int v = 16 / (int)esize(c->dtype);
-    if (!aligned(q, 16) || !aligned(out, 16) || q_bs % v || q_hs % v || o_bs % v || o_hs % v)
+    if (!paged_aligned(q, v, {c->B, q_bs}, {H, q_hs}) || !paged_aligned(out, v, {c->B, o_bs}, {H, o_hs}))
         return fail(SK_ERR_MISALIGNED, "sk_paged_attn: q, out and their strides must be 16-byte aligned");
     SK_REQUIRE(paged_apart(c->D, {c->B, o_bs}, {H, o_hs}) && (c->mass == nullptr || paged_book_apart(*c, c->mass_bs, c->mass_hs)),
                "sk_paged_attn: rows of out or mass overlap");
