@@ -4,7 +4,8 @@
 // last slot to be kept is found by four histograms of eight bits, summed over the cluster, and equal keys go by slot.  Then every slot
 // is kept or not, and the i-th freed slot below the budget and the i-th kept one behind it are written side by side.  A
 // list entry is a row of K, a row of V, a mass and a position to move; sources lie behind the budget and targets below it, so the
-// cluster's blocks move entries in any order once the list is complete.  Only what moves is read: mass and positions once, 241 of 4352 keys of D elements.
+// cluster's blocks move entries in any order once the list is complete.  Of keys and values only what moves is read, 241 of 4352 rows; positions once and
+// masses twice (the second time from L2), where a block's slots find room on chip.
 //
 // Measured, 8 heads of 128: 32 sequences from 4352 to 4096 slots 26.7 us (about 14 in passes of three barriers each, then 63 MB of rows), one from
 // 32768 to 4096 25.7 us (13 until its moves begin: passes end in barriers of the cluster).  Always four passes: 28.2 and 28; list and table read when
@@ -12,6 +13,7 @@
 // a kernel of their own 3 more, and a launch; with three histograms of 2048 bins 29 and 52, words of other blocks cost that much.
 #include "paged.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace sk {
@@ -363,6 +365,39 @@ paged_evict_lengths_kernel(const __grid_constant__ sk_paged_cache c, int budget,
     if (b < c.B) lengths_out[b] = min(paged_length(c, b, 0), budget);
 }
 
+// Do clusters of 16 blocks, more than every GPU takes, find a place on this device with all the shared memory that a block may have: asked of
+// the driver once per device
+bool ev_sixteen() {
+    constexpr int MAX_DEV = 64;
+    static std::atomic<int> known[MAX_DEV];                    // 0: not asked yet, 1: no, 2: yes
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEV) {
+        cudaGetLastError();
+        return false;
+    }
+    if (const int k = known[dev].load(std::memory_order_relaxed)) return k == 2;
+    auto kern = paged_evict_kernel<EV_CLUSTER>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(EV_CLUSTER);
+    cfg.blockDim = dim3(EV_THREADS);
+    cfg.dynamicSmemBytes = (size_t)EV_SLOTS * 8;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = EV_CLUSTER;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SLOTS * 8) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();                                    // no such clusters then, and no error of the next launch
+        n = 0;
+    }
+    known[dev].store(n > 0 ? 2 : 1, std::memory_order_relaxed);
+    return n > 0;
+}
+
 struct EvPlan {
     int cluster, room, most_moves;
     size_t total;                                              // bytes of the lists
@@ -372,13 +407,15 @@ EvPlan ev_plan(const sk_paged_cache& c, int budget) {
     const int64_t rows = (int64_t)c.B * c.G, cap = (int64_t)c.width * c.page;
     // Blocks of a row: twice as many while they find a place at once, two an SM, and then have four slots a thread; more where a block's slots have no
     // room on chip.  Sixteen come later, with eight slots a thread (one row of 65536 slots 26 us by 16 and 34 by 8, eight of 32768 29 and 26), and for
-    // more rows than half fill the GPU only where eight would not share SMs (16 rows of 131072 slots 192 and 281, of 70000 117 and 104)
+    // more rows than half fill the GPU only where eight would not share SMs (16 rows of 131072 slots 192 and 281, of 70000 117 and 104).  Where the
+    // device has no place for sixteen, eight do it too: slots without room on chip are read again
     p.cluster = 1;
     while (p.cluster < EV_CLUSTER) {
         const bool find_places = rows * 2 * p.cluster <= 2 * sm_count(), sixteen = p.cluster == 8;
         const bool pays = !sixteen ? cap >= (int64_t)8 * EV_THREADS * p.cluster
                                    : cap >= (int64_t)16 * EV_THREADS * 8 && (rows * 16 <= sm_count() || cap > (int64_t)EV_SLOTS_OF_TWO * 8);
         if (!(find_places && pays) && (cap + p.cluster - 1) / p.cluster <= EV_SLOTS) break;
+        if (sixteen && !ev_sixteen()) break;
         p.cluster *= 2;
     }
     const int64_t share = (cap + p.cluster - 1) / p.cluster;
@@ -395,10 +432,6 @@ int evict_launch(const sk_paged_cache& c, int budget, int recent, int sink, floa
     static SmemLimit limit;
     cudaError_t e = limit.raise((const void*)paged_evict_kernel<CL>, (size_t)EV_SLOTS * 8);
     if (e != cudaSuccess) return check_chained(e, "paged_evict_kernel");
-    if (CL > 8) {                                              // more than every GPU takes
-        e = cudaFuncSetAttribute((const void*)paged_evict_kernel<CL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return check_chained(e, "paged_evict_kernel");
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(c.B * c.G * CL));
     cfg.blockDim = dim3(EV_THREADS);
