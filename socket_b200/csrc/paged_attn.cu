@@ -12,7 +12,7 @@
 // The second kernel also adds the weights to mass, from scores that the first one leaves behind (they need the final maximum and sum).
 //
 // Measured, 32 / 8 heads of 128: 32768 keys 29 us (134 MB; first kernel 26 at 5.1 TB/s, the start and end of a block's run 5 of them), 4 x 131072 with
-// mass 376 us (350 at 6.3 TB/s and 25), 64 sequences of 1 to 8003 with mass 57.5 us (49 and 8).  Eight warps a block and one block an SM: two blocks of
+// mass 375 us (350 at 6.3 TB/s and 25), 64 sequences of 1 to 8003 with mass 57.7 us (49 and 8; fp16 59.0).  Eight warps a block and one block an SM: two blocks of
 // four cost the ragged batch 2 us and the long one 4.  A pair's end counted as one chunk: as two 3 us more, with work measured in tiles 1 to 50.
 //
 // 16-bit types: S^T = K Q^T and O^T = V^T P^T by m16n8k16 products, keys and then value columns in the 16 rows and up to 8 query heads in
@@ -31,8 +31,8 @@ constexpr int PT_KEYS = 16;                                    // keys of a warp
 // the sums mind, and the six exchanges and the rescaling that a rise takes are left out of nearly every tile.
 constexpr float PT_SLACK = 8.f;
 // fp16: raised to PT16_BELOW under the maximum, for a score PT16_SLACK above that.  Weights then reach 2^15 of a largest half of 65504, and only those
-// 20 powers of two under a maximum are small.  64 sequences of 1 to 8003 with mass 59.4 us, 58.0 with small weights lost; 4 x 131072 keys 348, of which
-// all but one are small 373, and 397 where they take two turns (344, all lost)
+// 20 powers of two under a maximum are small.  64 sequences of 1 to 8003 with mass, as called, 59.4 us, 58.0 with small weights lost; 4 x 131072 keys 348,
+// of which all but one are small 373, and 397 where they take two turns (344, all lost)
 constexpr float PT16_BELOW = 11.f, PT16_SLACK = 4.f, PT16_SMALL = 0x1p-9f, PT16_UP = 0x1p24f;
 
 template <typename T, int DP_, int NT_> struct PtShape {
@@ -727,7 +727,8 @@ paged_join_kernel(const __grid_constant__ sk_paged_cache c, const __grid_constan
                 const int64_t begin = flat - p.chunk + (int64_t)grp * (p.chunks + PT_PAD);
                 const int y0 = (int)pt_div(begin, per), y1 = (int)pt_div(begin + p.chunks - 1, per);
                 const float* sc = a.scores + begin * CHUNK * a.rs;
-                // four heads a key: the first keys' scores and masses are asked for before the heads' maxima are
+                // four heads a key: the first keys' scores and masses are asked for before the heads' maxima are, of four keys at a time (64 ragged
+                // sequences 59.0 us, key by key as with other numbers of heads 63.7; 4 x 131072 keys 375 and 407)
                 float4 x[4];
                 float w[4];
                 auto ask = [&](int j) {

@@ -177,7 +177,11 @@ def evict(k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, mass
 @dataclass(frozen=True)
 class Paging:
     """How a decoder keeps its caches in pages.  With a budget, sequences that have grown `every` tokens beyond it are cut back to
-    it: the first `sink` tokens, the last `recent` ones and the keys that decoded tokens attended to most stay."""
+    it: the first `sink` tokens, the last `recent` ones and the keys that decoded tokens attended to most stay.
+
+    A prompt's queries collect no weights.  One longer than `budget + every` is cut behind the first decoded token, by that token's
+    weights alone, and a later turn's tokens start from nothing beside keys that have collected for long: what has to outlast
+    that is `sink`'s and `recent`'s to keep."""
     page: int = 64
     pages: int = 0                      # of the pool; 0: as many as all sequences need at their longest
     budget: int = 0                     # 0: nothing is evicted
