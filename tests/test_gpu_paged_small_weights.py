@@ -71,3 +71,26 @@ def test_small_weights_of_other_heads(at, G, rep, D, dtype):
 @pytest.mark.parametrize("gap,value", [(17.5, 0.0), (18.0, 1.0), (24.0, 0.0)])
 def test_small_weights_of_a_long_cache(gap, value, dtype):
     _case([131072], 1, 4, 128, dtype, gap, 0, True, value)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1e3, 1e5, 3e6, 3e7, 6e7, 1e8, 2e8, 5e8, 2e9])
+def test_huge_scores_give_weights_all_the_same(size, dtype):
+    """Scores so large that fp32 has them in steps of up to 256: whatever they round to, weights are at most one and add up to one, so
+    a result is finite and lies among the values."""
+    lengths = [1, 16, 17, 300, 3000]
+    c = Cache(lengths, 1, 64, 16, dtype, DEV, seed=2)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q = torch.zeros(len(lengths), 4, 64, device=DEV)
+    q[..., 0], q[..., 1] = size / 6e4, 1.0                    # keys differ by what their second column adds: less than a step, or a few
+    for b, n in enumerate(lengths):
+        k = torch.zeros(1, n, 64, device=DEV)
+        k[..., 0], k[..., 1] = 6e4, torch.randint(-60, 60, (1, n), generator=g, device=DEV).float()
+        c.set(c.k, b, 0, k.to(dtype))
+    mass = torch.zeros(len(lengths), 1, c.cap, device=DEV)
+    out = paged.attn(q.to(dtype), *c.tensors, scale=1.0, mass=mass)
+    for b, n in enumerate(lengths):
+        v = c.get(c.v, b, n)[0].double()
+        low, high = v.amin(0) - 2.0 ** -7 * v.abs().amax(0), v.amax(0) + 2.0 ** -7 * v.abs().amax(0)
+        assert ((out[b].double() >= low) & (out[b].double() <= high)).all()
+        assert (mass[b] >= 0).all() and (mass[b].sum() - 4).abs() <= 4 * (n + 64) * 2.0 ** -23
